@@ -56,4 +56,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("flash_prefill", &kvs::flash_prefill);
   m.def("paged_decode_splits", &kvs::paged_decode_splits);
   m.def("paged_decode_attention", &kvs::paged_decode_attention);
+  // tree-drafted decoding
+  m.def("plan_step", &kvs::plan_step);
+  m.def("paged_tree_attention", &kvs::paged_tree_attention);
+  m.def("process_logits", &kvs::process_logits);
+  m.def("commit_tree", &kvs::commit_tree);
 }

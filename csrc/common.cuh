@@ -180,6 +180,7 @@ enum Status : uint32_t {
   kStatusBadSymbol = 3,
   kStatusBadSize = 4,
   kStatusPeerTimeout = 5,  // a tensor-parallel peer's tile or flag did not arrive in time
+  kStatusNoBlocks = 6,     // the free list holds fewer KV blocks than a step plan needs
 };
 
 }  // namespace kvs

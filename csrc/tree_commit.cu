@@ -1,0 +1,212 @@
+// Greedy verification of a drafted tree and commit of the accepted path.
+//
+// Node 0 of a request's tree is its last chosen token, which is certain.
+// From cur = 0: while a child c of cur (the lowest one) carries the token that
+// the model chose after cur (draft[c] == target[cur]), cur = c.  The nodes
+// passed are the path; the model's choice after the last one is the next
+// token.  The K/V rows of the path go from the step's staging rows to the
+// cache slots of positions ctx, ctx + 1, ..., for every layer in one launch.
+//
+// Each row of K or V is read and written once: bound by HBM for a full batch
+// and by latency for a single request.  One CTA per (layer and part, request)
+// repeats the walk (a few hundred bytes that stay in L1) instead of waiting
+// for another launch to write the path down.
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include "common.cuh"
+#include "ops.h"
+
+namespace kvs {
+namespace {
+
+constexpr int kCommitThreads = 256;
+constexpr int kMaxTree = 1024;
+
+struct CommitArgs {
+  const int32_t *drafts, *targets, *parents, *indptr, *ctx, *slots;
+  int R;
+  const uint4* src;  // staging rows [L, 2, R, Hkv, D], strides in 16-byte words
+  int64_t src_l, src_p, src_r, src_h;
+  uint4* dst;  // cache [L, 2, blocks, bs, Hkv, D]
+  int64_t dst_l, dst_p, dst_b, dst_t, dst_h;
+  int layers, heads, words, bs;  // words: 16-byte words of one head's row
+  int64_t num_slots;
+  int32_t* tokens;
+  int64_t tokens_stride;
+  int tokens_len;
+  int32_t *accepted, *path, *next, *ctx_out;
+  uint32_t* status;
+};
+
+// Walk of one request by one warp; s_path receives the node of each step.
+__device__ __forceinline__ int walk(const CommitArgs& a, int lo, int n, int lane, uint16_t* s_path) {
+  int len = 0, cur = 0;
+  if (n <= 0) return 0;
+  while (true) {
+    if (lane == 0) s_path[len] = uint16_t(cur);
+    ++len;
+    const int want = a.targets[lo + cur];
+    int child = n;
+    if (a.parents == nullptr) {
+      if (cur + 1 < n && a.drafts[lo + cur + 1] == want) child = cur + 1;
+    } else {
+      for (int base = (cur + 1) & ~31; base < n; base += 32) {
+        const int i = base + lane;
+        const bool is = i > cur && i < n && a.parents[lo + i] == cur && a.drafts[lo + i] == want;
+        const unsigned hit = __ballot_sync(0xffffffffu, is);
+        if (hit) {
+          child = base + __ffs(hit) - 1;
+          break;
+        }
+      }
+    }
+    if (child >= n) break;
+    cur = child;  // indices only grow, so the walk ends
+  }
+  __syncwarp();
+  return len;
+}
+
+__global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(CommitArgs a) {
+  pdl_trigger();
+  __shared__ uint16_t s_path[kMaxTree];
+  __shared__ int s_len;
+  const int b = blockIdx.y, lp = blockIdx.x;
+  const int lo = min(max(a.indptr[b], 0), a.R), hi = min(max(a.indptr[b + 1], lo), a.R);
+  const int n = min(hi - lo, kMaxTree);
+  if (threadIdx.x < 32) {
+    const int len = walk(a, lo, n, threadIdx.x, s_path);
+    if (threadIdx.x == 0) s_len = len;
+  }
+  __syncthreads();
+  const int len = s_len;
+  if (lp == 0) {
+    const int ctx = a.ctx[b];
+    for (int k = threadIdx.x; k < hi - lo; k += kCommitThreads) {
+      a.path[lo + k] = k < len ? int(s_path[k]) : -1;
+      if (k < len && a.tokens != nullptr) {
+        const int64_t at = int64_t(ctx) + k;
+        if (at >= 0 && at < a.tokens_len)
+          a.tokens[b * a.tokens_stride + at] = a.drafts[lo + s_path[k]];
+        else
+          atomicCAS(a.status, 0u, uint32_t(kStatusBadSize));
+      }
+    }
+    if (threadIdx.x == 0) {
+      a.accepted[b] = len;
+      a.next[b] = len > 0 ? a.targets[lo + s_path[len - 1]] : -1;
+      a.ctx_out[b] = ctx + len;
+      if (hi - lo > kMaxTree) atomicCAS(a.status, 0u, uint32_t(kStatusBadSize));
+    }
+    if (b == 0)  // rows past the last request
+      for (int r = min(max(a.indptr[gridDim.y], 0), a.R) + threadIdx.x; r < a.R; r += kCommitThreads) a.path[r] = -1;
+  }
+  if (a.src == nullptr) return;
+  const uint4* src = a.src + (lp >> 1) * a.src_l + (lp & 1) * a.src_p;
+  uint4* dst = a.dst + (lp >> 1) * a.dst_l + (lp & 1) * a.dst_p;
+  const int row = a.heads * a.words;
+  for (int e = threadIdx.x; e < len * row; e += kCommitThreads) {
+    const int k = e / row, c = e % row, h = c / a.words, w = c % a.words;
+    const int slot = a.slots[lo + k];
+    if (slot < 0 || slot >= a.num_slots) {
+      atomicCAS(a.status, 0u, uint32_t(kStatusBadSize));
+      continue;
+    }
+    dst[(slot / a.bs) * a.dst_b + (slot % a.bs) * a.dst_t + h * a.dst_h + w] =
+        src[(lo + s_path[k]) * a.src_r + h * a.src_h + w];
+  }
+}
+
+}  // namespace
+
+void commit_tree(torch::Tensor draft_ids, torch::Tensor target_ids, c10::optional<torch::Tensor> parents,
+                 torch::Tensor indptr, torch::Tensor ctx_lens, torch::Tensor slot_mapping,
+                 c10::optional<torch::Tensor> tree_kv, c10::optional<torch::Tensor> kv_cache,
+                 c10::optional<torch::Tensor> tokens, torch::Tensor accepted, torch::Tensor path,
+                 torch::Tensor next_ids, torch::Tensor ctx_out, torch::Tensor status) {
+  const int64_t R = draft_ids.numel(), B = ctx_lens.numel();
+  auto vec = [&](const torch::Tensor& t, int64_t n, const char* msg) {
+    KVS_CHECK_ARG(t.is_cuda() && t.dim() == 1 && t.is_contiguous() && t.scalar_type() == at::kInt &&
+                      t.numel() == n && t.device() == draft_ids.device(),
+                  msg);
+  };
+  const char* rows = "commit_tree: draft_ids, target_ids, parents, slot_mapping, path are int32 [R] on one CUDA device";
+  const char* reqs = "commit_tree: ctx_lens, accepted, next_ids are int32 [B], indptr [B + 1]";
+  vec(draft_ids, R, rows);
+  vec(target_ids, R, rows);
+  vec(slot_mapping, R, rows);
+  vec(path, R, rows);
+  if (parents.has_value()) vec(*parents, R, rows);
+  vec(indptr, B + 1, reqs);
+  vec(ctx_lens, B, reqs);
+  vec(accepted, B, reqs);
+  vec(next_ids, B, reqs);
+  vec(ctx_out, B, reqs);
+  KVS_CHECK_ARG(B >= 1 && B <= 65535, "commit_tree: 1 to 65535 requests");
+  KVS_CHECK_ARG(R < (int64_t(1) << 30), "commit_tree: too many rows");
+  KVS_CHECK_ARG(tree_kv.has_value() == kv_cache.has_value(), "commit_tree: tree_kv and kv_cache go together");
+  CommitArgs a{};
+  if (tokens.has_value()) {
+    KVS_CHECK_ARG(tokens->is_cuda() && tokens->dim() == 2 && tokens->size(0) == B && tokens->stride(1) == 1 &&
+                      tokens->scalar_type() == at::kInt && tokens->device() == draft_ids.device(),
+                  "commit_tree: tokens [B, M] int32 with contiguous rows");
+    a.tokens = tokens->data_ptr<int32_t>();
+    a.tokens_stride = tokens->stride(0);
+    a.tokens_len = int(std::min<int64_t>(tokens->size(1), INT32_MAX));
+  }
+  int64_t planes = 1;
+  if (tree_kv.has_value() && R > 0) {
+    const torch::Tensor &s = *tree_kv, &c = *kv_cache;
+    KVS_CHECK_ARG(s.is_cuda() && c.is_cuda() && s.dim() == 5 && c.dim() == 6 && s.scalar_type() == c.scalar_type() &&
+                      s.device() == draft_ids.device() && c.device() == draft_ids.device(),
+                  "commit_tree: tree_kv [L, 2, R, Hkv, D] and kv_cache [L, 2, blocks, block_size, Hkv, D] of one type");
+    KVS_CHECK_ARG(s.size(0) == c.size(0) && s.size(1) == 2 && c.size(1) == 2 && s.size(2) >= R &&
+                      s.size(3) == c.size(4) && s.size(4) == c.size(5) && s.size(0) >= 1,
+                  "commit_tree: tree_kv and kv_cache shapes differ");
+    const int64_t item = s.element_size();
+    bool wide = s.stride(4) == 1 && c.stride(5) == 1 && (s.size(4) * item) % 16 == 0 &&
+                (reinterpret_cast<uintptr_t>(s.data_ptr()) & 15) == 0 &&
+                (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15) == 0;
+    for (int d = 0; d < 4; ++d) wide = wide && (s.stride(d) * item) % 16 == 0;
+    for (int d = 0; d < 5; ++d) wide = wide && (c.stride(d) * item) % 16 == 0;
+    KVS_CHECK_ARG(wide, "commit_tree: head rows must be contiguous multiples of 16 bytes at 16-byte boundaries");
+    a.src = reinterpret_cast<const uint4*>(s.data_ptr());
+    a.dst = reinterpret_cast<uint4*>(c.data_ptr());
+    auto words = [&](int64_t stride) { return stride * item / 16; };
+    a.src_l = words(s.stride(0));
+    a.src_p = words(s.stride(1));
+    a.src_r = words(s.stride(2));
+    a.src_h = words(s.stride(3));
+    a.dst_l = words(c.stride(0));
+    a.dst_p = words(c.stride(1));
+    a.dst_b = words(c.stride(2));
+    a.dst_t = words(c.stride(3));
+    a.dst_h = words(c.stride(4));
+    a.layers = int(s.size(0));
+    a.heads = int(s.size(3));
+    a.words = int(s.size(4) * item / 16);
+    a.bs = int(c.size(3));
+    a.num_slots = c.size(2) * c.size(3);
+    KVS_CHECK_ARG(int64_t(a.heads) * a.words * kMaxTree <= INT32_MAX, "commit_tree: K/V rows too long");
+    planes = s.size(0) * 2;
+  }
+  const c10::cuda::CUDAGuard guard(draft_ids.device());
+  a.drafts = draft_ids.data_ptr<int32_t>();
+  a.targets = target_ids.data_ptr<int32_t>();
+  a.parents = parents.has_value() ? parents->data_ptr<int32_t>() : nullptr;
+  a.indptr = indptr.data_ptr<int32_t>();
+  a.ctx = ctx_lens.data_ptr<int32_t>();
+  a.slots = slot_mapping.data_ptr<int32_t>();
+  a.R = int(R);
+  a.accepted = accepted.data_ptr<int32_t>();
+  a.path = path.data_ptr<int32_t>();
+  a.next = next_ids.data_ptr<int32_t>();
+  a.ctx_out = ctx_out.data_ptr<int32_t>();
+  a.status = reinterpret_cast<uint32_t*>(status.data_ptr<int32_t>());
+  tree_commit_kernel<<<dim3(unsigned(planes), unsigned(B)), kCommitThreads, 0, at::cuda::getCurrentCUDAStream()>>>(a);
+  KVS_CUDA_CHECK(cudaGetLastError());
+}
+
+}  // namespace kvs

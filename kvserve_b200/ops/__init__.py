@@ -17,10 +17,12 @@ from ._ext import ext, available, ExtensionMissing
 __all__ = [
     "ext", "available", "ExtensionMissing", "linear", "gemm", "gemv", "rmsnorm", "rope_qkv",
     "silu_mul", "gemm_silu", "gemm_qkv_rope", "interleave_gate_up", "GATE_UP_BLOCK", "embedding", "argmax", "flash_prefill", "paged_decode_attention",
-    "device_status", "check_device_status", "STATUS_NAMES",
+    "device_status", "check_device_status", "STATUS_NAMES", "StepPlan", "TreeCommit", "plan_step", "paged_tree_attention",
+    "process_logits", "commit_tree",
 ]
 
-STATUS_NAMES = {0: "ok", 1: "timeout", 2: "bad header", 3: "bad symbol", 4: "bad size"}
+STATUS_NAMES = {0: "ok", 1: "timeout", 2: "bad header", 3: "bad symbol", 4: "bad size",
+                5: "peer timeout", 6: "no free KV blocks"}
 GEMV_MAX_M = 8
 
 _status: dict[int, torch.Tensor] = {}
@@ -242,3 +244,6 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     ext().paged_decode_attention(q, k_cache, v_cache, block_tables, ctx_lens, max_ctx, scale, out,
                                  part_o, part_ml, splits)
     return out
+
+
+from .tree import StepPlan, TreeCommit, commit_tree, paged_tree_attention, plan_step, process_logits  # noqa: E402

@@ -27,6 +27,10 @@ SOURCES = [
     "attention_decode.cu",
     "paged_decode_noalloc.cu",
     "p2p.cu",
+    "step_plan.cu",
+    "tree_attention.cu",
+    "logits_rules.cu",
+    "tree_commit.cu",
 ]
 
 NVCC_FLAGS = [

@@ -4,6 +4,7 @@
 #include <torch/extension.h>
 
 #include "ops.h"
+#include "tree_ops.h"
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "kvserve_b200 sm_100a kernels";

@@ -12,7 +12,7 @@
 #include <c10/cuda/CUDAGuard.h>
 
 #include "common.cuh"
-#include "ops.h"
+#include "tree_ops.h"
 
 namespace kvs {
 namespace {

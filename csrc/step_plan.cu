@@ -20,7 +20,7 @@
 #include <cooperative_groups.h>
 
 #include "common.cuh"
-#include "ops.h"
+#include "tree_ops.h"
 
 namespace kvs {
 namespace {

@@ -104,9 +104,9 @@ def paged_tree_attention(q: torch.Tensor, k_tree: torch.Tensor, v_tree: torch.Te
         scale = 1.0 / math.sqrt(q.shape[-1])
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    count_launches(1)
+    count_launches(2)
     ext().paged_tree_attention(q, k_tree, v_tree, k_cache, v_cache, block_tables, ctx_lens, indptr, tree_mask,
-                               float(scale), out)
+                               float(scale), out, device_status(q.device))
     return out
 
 

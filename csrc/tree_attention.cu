@@ -31,7 +31,7 @@ namespace {
 
 constexpr int BM = 128;      // query rows of a tile (the MMA's M)
 constexpr int BN = 64;       // tokens of a K/V tile
-constexpr int kThreads = 192;  // warps 0..3 softmax, 4 loader, 5 MMA issuer
+constexpr int kThreads = 448;  // warps 0..3 and 4..7 softmax of the two streams, 8 and 9 loaders, 10..13 MMA issuers
 constexpr float kRescaleThreshold = 8.0f;  // log2: P stays below 2^8 between rescalings
 
 struct TreeArgs {
@@ -44,19 +44,23 @@ struct TreeArgs {
   int width, words, R, B, hkv, group, bs;
   int box;         // tokens of one TMA box of the cache (0: rows are copied by the loader warp)
   bool tree_tma;   // tree rows by TMA
+  bool q_tma;      // query rows by TMA
+  int q_box;       // tree nodes of one TMA box of q
+  int nodes;       // tree nodes of a row tile (nodes * group <= BM)
   bool k_head_first, v_head_first, kt_head_first, vt_head_first;  // order of the middle tensor-map dimensions
   int min_share;
+  int ctas;
   int part_rows;   // rows kept per partial record
   float scale_log2;
-  float* part_o;    // [2 * CTAs, part_rows, D]
-  float2* part_ml;  // [2 * CTAs, part_rows]
+  float* part_o;    // [4 * CTAs, part_rows, D]
+  float2* part_ml;  // [4 * CTAs, part_rows]
   int64_t* base;    // [B + 1] first tile of each request, then the share
   uint32_t* err;
 };
 
 // ------------------------------------------------------------------ schedule
 struct Shape {  // of one request
-  int lo, n, ctx, nt_ctx, nt, mt;
+  int lo, n, ctx, nt_ctx, nt, mt, pairs;
 };
 __device__ __forceinline__ Shape request_shape(const TreeArgs& a, int b) {
   Shape s;
@@ -64,18 +68,22 @@ __device__ __forceinline__ Shape request_shape(const TreeArgs& a, int b) {
   s.n = max(min(a.indptr[b + 1], a.R) - s.lo, 0);
   s.ctx = int(max(min(int64_t(a.ctx[b]), int64_t(a.width) * a.bs), int64_t(0)));
   s.nt_ctx = (s.ctx + BN - 1) / BN;
-  s.mt = int((int64_t(s.n) * a.group + BM - 1) / BM);
+  s.mt = (s.n + a.nodes - 1) / a.nodes;
+  s.pairs = (s.mt + 1) / 2;
   s.nt = s.n > 0 ? s.nt_ctx + (s.n + BN - 1) / BN : 0;
   return s;
 }
-// Row tiles of one KV head read the same K/V.  Items with several row tiles
-// are cut into segments of at least one CTA share and ordered (segment, row
-// tile), so the CTAs that read one segment run side by side and all but the
-// first find it in L2.
+__device__ __forceinline__ int64_t tile_count(const TreeArgs& a, const Shape& s) {
+  return int64_t(a.hkv) * s.pairs * s.nt;
+}
+// The pairs of row tiles of one KV head read the same K/V.  Items with
+// several pairs are cut into segments of at least one CTA share and ordered
+// (segment, pair), so the CTAs that read one segment run side by side and all
+// but the first find it in L2.
 struct Segments {
   int count, len, longer;  // `longer` segments of len + 1 tiles, then segments of len
   __device__ __forceinline__ Segments(const Shape& s, int64_t share) {
-    count = s.mt > 1 ? int(max(int64_t(1), int64_t(s.nt) / share)) : 1;
+    count = s.pairs > 1 ? int(max(int64_t(1), int64_t(s.nt) / share)) : 1;
     len = s.nt / count;
     longer = s.nt % count;
   }
@@ -83,12 +91,16 @@ struct Segments {
   __device__ __forceinline__ int start(int i) const { return i * len + min(i, longer); }
 };
 
-struct Piece {  // consecutive tiles of one item
+struct Piece {  // consecutive tiles of one item (request, KV head, pair of row tiles)
   Shape s;
-  int b, h, mi;
-  int t0, t1;    // tiles [t0, t1) of the item
-  bool starts;   // begins its segment
-  bool whole;    // the complete item
+  int b, h, pair;
+  int t0, t1;     // tiles [t0, t1) of the item
+  bool starts;    // begins its segment
+  bool whole;     // the complete item
+  bool two;       // the pair has two row tiles: each stream takes one; else the streams take turns in tiles
+  __device__ __forceinline__ int rows(const TreeArgs& a, int k) const {
+    return min(s.n - (2 * pair + k) * a.nodes, a.nodes) * a.group;
+  }
 };
 
 struct Walker {  // the pieces of one CTA's share, in order
@@ -97,30 +109,31 @@ struct Walker {  // the pieces of one CTA's share, in order
   Shape s;
   __device__ __forceinline__ bool next(const TreeArgs& a, Piece& p) {
     if (at >= end) return false;
-    while (at >= base + int64_t(a.hkv) * s.mt * s.nt) {
-      base += int64_t(a.hkv) * s.mt * s.nt;
+    while (at >= base + tile_count(a, s)) {
+      base += tile_count(a, s);
       s = request_shape(a, ++b);
     }
     const Segments seg(s, share);
     const int64_t x = at - base;
-    const int64_t per_head = int64_t(s.mt) * s.nt;
+    const int64_t per_head = int64_t(s.pairs) * s.nt;
     p.s = s;
     p.b = b;
     p.h = int(x / per_head);
     const int64_t y = x - p.h * per_head;
-    const int64_t big = int64_t(seg.len + 1) * s.mt;
+    const int64_t big = int64_t(seg.len + 1) * s.pairs;
     int i;
     if (y < big * seg.longer) i = int(y / big);
-    else i = seg.longer + int((y - big * seg.longer) / (int64_t(seg.len) * s.mt));
-    const int64_t z = y - int64_t(seg.start(i)) * s.mt;
+    else i = seg.longer + int((y - big * seg.longer) / (int64_t(seg.len) * s.pairs));
+    const int64_t z = y - int64_t(seg.start(i)) * s.pairs;
     const int len = seg.length(i);
-    p.mi = int(z / len);
-    const int off = int(z - int64_t(p.mi) * len);
+    p.pair = int(z / len);
+    const int off = int(z - int64_t(p.pair) * len);
     const int take = int(min(int64_t(len - off), end - at));
     p.t0 = seg.start(i) + off;
     p.t1 = p.t0 + take;
     p.starts = off == 0;
     p.whole = take == s.nt;
+    p.two = 2 * p.pair + 1 < s.mt;
     at += take;
     return true;
   }
@@ -180,7 +193,16 @@ __device__ __forceinline__ void add2(float& s0, float& s1, float a0, float a1) {
       : "+f"(s0), "+f"(s1)
       : "f"(a0), "f"(a1));
 }
-__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{.reg .pred q;\n.reg .b32 r;\nelect.sync r|q, 0xffffffff;\nselp.u32 %0, 1, 0, q;}" : "=r"(p));
+  return p != 0;
+}
+// Named barriers: 1 and 2 the warpgroup of stream 0 and 1 (128 threads), 3
+// both on a shared V tile, 4 both at the end of a piece (256).
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const void* map, int c0, int c1, int c2, uint64_t* bar) {
   asm volatile(
@@ -204,19 +226,30 @@ __device__ __forceinline__ uint32_t tile_offset(int rows, int r, int c) {
   return uint32_t(c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
+struct Shared {
+  float2 ml[2][BM];       // row maximum and sum of the two streams
+  int64_t sum[kThreads / 32], base;
+  int b;
+  uint32_t tmem;
+  uint32_t odd[4];        // 1 + the last unit whose tree V held values that are not finite
+  uint32_t piece_odd[2];  // ... in the streams' tiles of the piece
+};
+
 template <int D>
 struct Layout {
-  static constexpr int STAGES = D == 128 ? 2 : 4;
+  static constexpr int STAGES = D == 128 ? 5 : 10;
   static constexpr int PANELS = D / 64;
   static constexpr int Q_BYTES = BM * D * 2;
   static constexpr int TILE = BN * D * 2;
-  static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + STAGES * TILE, OFF_BAR = OFF_V + STAGES * TILE;
-  // barriers: k_full, k_empty, v_full, v_empty [STAGES] each, s_full[2],
-  // p_full[2], pv_done[2], q_full, o_full
-  static constexpr int NUM_BARS = 4 * STAGES + 8;
-  static constexpr int SMEM = OFF_BAR + NUM_BARS * 8 + 1024;
-  static constexpr uint32_t TMEM_COLS = 256;  // S/P double buffered (2 x 64), O (D)
+  static constexpr int OFF_K = 2 * Q_BYTES, OFF_V = OFF_K + STAGES * TILE, OFF_BAR = OFF_V + STAGES * TILE;
+  // barriers: k_full, k_empty, v_full, v_empty [STAGES] each, s_full[4],
+  // p_full[4], pv_done[4], q_full[2], q_empty[2], o_full, o_empty, drain[4]
+  static constexpr int NUM_BARS = 4 * STAGES + 22;
+  static constexpr int OFF_SHARED = OFF_BAR + NUM_BARS * 8;
+  static constexpr int SMEM = OFF_SHARED + int(sizeof(Shared)) + (D == 128 ? 0 : 1024);
+  static constexpr uint32_t TMEM_COLS = 512;  // S/P of 4 units (64 each), O of 2 streams (128 each)
 };
+static_assert(Layout<128>::SMEM <= 232448 && Layout<64>::SMEM <= 232448, "shared memory of one SM");
 
 // Copies the rows of one K or V tile with plain loads (one warp): caches
 // whose blocks TMA boxes do not tile.  Rows at or past `valid` become zero.
@@ -247,51 +280,77 @@ __device__ __forceinline__ void copy_paged_tile(uint8_t* dst, const uint16_t* ca
   }
 }
 
+// One CTA per SM.  A unit is one row tile against one K/V tile:
+//   S(u) = Q K^T -> softmax -> P(u) over S(u) in TMEM -> O += P(u) V.
+// Units alternate between two streams (u mod 2), each with its own softmax
+// warpgroup and O accumulator, so one stream's softmax runs under the other's
+// products; S has four buffers, so a stream's softmax does not wait for its
+// own products either.  An item with two row
+// tiles gives each stream one of them (a K/V tile feeds both); with one row
+// tile the streams take turns in its K/V tiles and are joined at the end.
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, 1)
     tree_attention_kernel(const __grid_constant__ CUtensorMap m_kc, const __grid_constant__ CUtensorMap m_vc,
                           const __grid_constant__ CUtensorMap m_kt, const __grid_constant__ CUtensorMap m_vt,
-                          const TreeArgs a) {
+                          const __grid_constant__ CUtensorMap m_q, const TreeArgs a) {
   using Lay = Layout<D>;
   using namespace sm100;
   constexpr int ST = Lay::STAGES;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // the tiles fill the SM, so the 1024-byte alignment that their swizzle needs
+  // is asked for instead of padded for, and checked
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023) {
+    if (threadIdx.x == 0) atomicCAS(a.err, 0u, uint32_t(kStatusBadSize));
+    return;
+  }
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Lay::OFF_BAR);
   uint64_t *k_full = bars, *k_empty = bars + ST, *v_full = bars + 2 * ST, *v_empty = bars + 3 * ST;
-  uint64_t *s_full = bars + 4 * ST, *p_full = s_full + 2, *pv_done = s_full + 4, *q_full = s_full + 6,
-           *o_full = s_full + 7;
-  __shared__ uint32_t s_tmem;
-  __shared__ int64_t s_sum[kThreads / 32];
-  __shared__ int64_t s_base;
-  __shared__ int s_b;
-  __shared__ uint32_t s_odd[2];  // 1 + number of the last tile whose tree V held values that are not finite
+  uint64_t *s_full = bars + 4 * ST, *p_full = s_full + 4, *pv_done = s_full + 8, *q_full = s_full + 12,
+           *q_empty = s_full + 14, *o_full = s_full + 16, *o_empty = s_full + 17,
+           *drain = s_full + 18;
+  Shared& sh = *reinterpret_cast<Shared*>(smem + Lay::OFF_SHARED);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_trigger();
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < Lay::NUM_BARS; ++i) mbar_init(&bars[i], 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&p_full[i], 4);  // one arrival per softmax warp
-    mbar_init(q_full, 128);
+    tma_prefetch_desc(&m_kc);
+    tma_prefetch_desc(&m_vc);
+    tma_prefetch_desc(&m_kt);
+    tma_prefetch_desc(&m_vt);
+    tma_prefetch_desc(&m_q);
+    for (int i = 0; i < Lay::NUM_BARS; ++i) {
+      uint64_t* bar = bars + i;
+      uint32_t arrivals = 1;
+      if ((bar >= k_empty && bar < k_empty + ST) || (bar >= v_empty && bar < v_empty + ST) ||
+          (bar >= q_empty && bar < q_empty + 2) || bar == o_full)
+        arrivals = 2;  // one for each stream
+      if (bar >= p_full && bar < p_full + 4) arrivals = 4;  // the warps of a stream
+      if (bar == o_empty) arrivals = 8;
+      mbar_init(bar, arrivals);
+    }
     fence_barrier_init();
-    s_odd[0] = s_odd[1] = 0;
+    for (int i = 0; i < 4; ++i) sh.odd[i] = 0;
   }
-  if (warp == 5) tmem_alloc<Lay::TMEM_COLS>(&s_tmem);
+  if (warp == 9) tmem_alloc<Lay::TMEM_COLS>(&sh.tmem);
 
-  // sum the tiles of all requests, twice: once for the total (and with it the
-  // share), once to find the request that this CTA's share begins in
+  // Sum the tiles of all requests for the total (and with it the share), and
+  // find the request that this CTA's share begins in; a second pass is needed
+  // only where the requests outnumber the threads.
   Walker walk;
   walk.share = 0;
-  int64_t total = 0;
   for (int pass = 0; pass < 2; ++pass) {
-    int64_t carry = 0;
+    int64_t carry = 0, from = 0, mine = 0;
+    auto settle = [&](int b) {
+      if (b >= a.B) return;
+      if (blockIdx.x == 0) a.base[b] = from;
+      if (walk.at >= from && walk.at < from + mine) {
+        sh.b = b;
+        sh.base = from;
+      }
+    };
     for (int b0 = 0; b0 < a.B; b0 += kThreads) {
       const int b = b0 + threadIdx.x;
-      int64_t mine = 0;
-      if (b < a.B) {
-        const Shape s = request_shape(a, b);
-        mine = int64_t(a.hkv) * s.mt * s.nt;
-      }
+      mine = b < a.B ? tile_count(a, request_shape(a, b)) : 0;
       int64_t x = mine;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -299,248 +358,314 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (lane >= d) x += y;
       }
       __syncthreads();
-      if (lane == 31) s_sum[warp] = x;
+      if (lane == 31) sh.sum[warp] = x;
       __syncthreads();
-      int64_t before = carry;
+      from = carry + x - mine;
 #pragma unroll
       for (int w = 0; w < kThreads / 32; ++w) {
-        before += w < warp ? s_sum[w] : 0;
-        carry += s_sum[w];
+        from += w < warp ? sh.sum[w] : 0;
+        carry += sh.sum[w];
       }
-      if (pass == 1 && b < a.B) {
-        const int64_t from = before + x - mine;
-        if (blockIdx.x == 0) a.base[b] = from;
-        if (walk.at >= from && walk.at < from + mine) {
-          s_b = b;
-          s_base = from;
-        }
-      }
+      if (pass == 1) settle(b);
     }
     if (pass == 0) {
-      total = carry;
-      walk.share = max((total + gridDim.x - 1) / int64_t(gridDim.x), int64_t(a.min_share));
+      walk.share = max((carry + gridDim.x - 1) / int64_t(gridDim.x), int64_t(a.min_share));
       walk.at = blockIdx.x * walk.share;
-      walk.end = min(walk.at + walk.share, total);
+      walk.end = min(walk.at + walk.share, carry);
+      if (a.B <= kThreads) {
+        settle(threadIdx.x);
+        break;
+      }
     }
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) a.base[a.B] = walk.share;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = s_tmem;
-  const uint32_t tO = tmem + 2 * BN;
+  const uint32_t tmem = sh.tmem;
+  const uint32_t tO = tmem + 4 * BN;  // O of stream s at tO + s * 128
   const bool busy = walk.at < walk.end;
   if (busy) {
-    walk.b = s_b;
-    walk.base = s_base;
+    walk.b = sh.b;
+    walk.base = sh.base;
     walk.s = request_shape(a, walk.b);
   }
   Piece p;
 
-  if (busy && warp == 4) {
-    // ------------------------------------------------------------- loader
+  if (busy && (warp == 8 || warp == 9)) {
+    // ------------------------------------------------------------ loaders
+    // Warp 8 loads Q and K, warp 9 loads V: one warp for both could not issue
+    // the 2 KB boxes of 16-token blocks as fast as HBM delivers them.
+    const bool is_v = warp == 9;
+    uint64_t *full = is_v ? v_full : k_full, *empty = is_v ? v_empty : k_empty;
+    uint8_t* ring = smem + (is_v ? Lay::OFF_V : Lay::OFF_K);
+    const CUtensorMap *m_c = is_v ? &m_vc : &m_kc, *m_t = is_v ? &m_vt : &m_kt;
+    const bool c_head_first = is_v ? a.v_head_first : a.k_head_first;
+    const bool t_head_first = is_v ? a.vt_head_first : a.kt_head_first;
     bool ok = true;
-    int g = 0;  // tiles so far, over all pieces
+    int g = 0, qc = 0;  // K/V tiles and Q tiles so far
+    // waits of the whole warp
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      ok = ok && mbar_wait(bar, parity, a.err);
+      ok = __all_sync(0xffffffffu, ok);
+      return ok;
+    };
+    auto publish = [&](uint64_t* bar) {  // after plain stores of the warp
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    const int lane_box = lane / Lay::PANELS, lane_c = lane % Lay::PANELS;  // lane = (box, panel of 64 columns)
     while (ok && walk.next(a, p)) {
       const int32_t* table = a.tables + p.b * a.table_stride;
-      for (int j = p.t0; j < p.t1 && ok; ++j, ++g) {
+      // block and offset of this lane's box in tile j
+      auto locate = [&](int j, int& blk, int& off) {
+        const int t = j * BN + lane_box * a.box;
+        if (j < p.s.nt_ctx && j < p.t1 && lane_box * a.box < BN && t < p.s.ctx) {
+          blk = table[t / a.bs];
+          off = t % a.bs;
+        }
+      };
+      int next_blk = 0, next_off = 0;
+      if (a.box > 0) locate(p.t0, next_blk, next_off);
+      for (int k = 0; !is_v && k <= int(p.two); ++k, ++qc) {
+        const int node0 = (2 * p.pair + k) * a.nodes, nodes = min(p.s.n - node0, a.nodes);
+        uint8_t* dq = smem + (qc & 1) * Lay::Q_BYTES;
+        if (!wait(&q_empty[qc & 1], ((qc >> 1) & 1) ^ 1)) break;
+        if (a.q_tma) {
+          const int boxes = (nodes + a.q_box - 1) / a.q_box, box_rows = a.q_box * a.group;
+          if (lane == 0) mbar_arrive_expect_tx(&q_full[qc & 1], uint32_t(boxes) * box_rows * D * 2);
+          __syncwarp();
+          if (lane < boxes)
+            for (int c = 0; c < Lay::PANELS; ++c)
+              tma_load_3d(dq + c * BM * 128 + lane * box_rows * 128, &m_q, c * 64, p.h * a.group,
+                          p.s.lo + node0 + lane * a.q_box, &q_full[qc & 1]);
+        } else {
+          const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q);
+          constexpr int C = D / 8;
+          for (int e = lane; e < nodes * a.group * C; e += 32) {
+            const int r = e / C, c = e % C, node = node0 + r / a.group, hg = r % a.group;
+            *reinterpret_cast<uint4*>(dq + tile_offset(BM, r, c)) = *reinterpret_cast<const uint4*>(
+                q + int64_t(p.s.lo + node) * a.q_r + int64_t(p.h * a.group + hg) * a.q_h + c * 8);
+          }
+          publish(&q_full[qc & 1]);
+        }
+      }
+      for (int j = p.t0; j < p.t1 && ok; ++j) {
         const int st = g % ST;
-        const uint32_t free_parity = ((g / ST) & 1) ^ 1;
-        uint8_t *dk = smem + Lay::OFF_K + st * Lay::TILE, *dv = smem + Lay::OFF_V + st * Lay::TILE;
+        uint8_t* dst = ring + st * Lay::TILE;
+        const int blk = next_blk, off = next_off;
+        if (a.box > 0) locate(j + 1, next_blk, next_off);
+        if (!wait(&empty[st], ((g / ST) & 1) ^ 1)) break;
         if (j < p.s.nt_ctx) {
           const int t0 = j * BN, valid = min(BN, p.s.ctx - t0);
           if (a.box > 0) {
             const int boxes = (valid + a.box - 1) / a.box;
-            int blk = 0, off = 0;
-            if (lane < boxes) {
-              const int t = t0 + lane * a.box;
-              blk = table[t / a.bs];
-              off = t % a.bs;
-            }
-            const uint32_t bytes = uint32_t(boxes) * a.box * D * 2;
-            ok = mbar_wait(&k_empty[st], free_parity, a.err);
-            if (lane == 0 && ok) mbar_arrive_expect_tx(&k_full[st], bytes);
-            ok = __all_sync(0xffffffffu, ok);
-            if (lane < boxes && ok)
-              for (int c = 0; c < Lay::PANELS; ++c)
-                tma_load_4d(dk + c * BN * 128 + lane * a.box * 128, &m_kc, c * 64, a.k_head_first ? p.h : off,
-                            a.k_head_first ? off : p.h, blk, &k_full[st]);
-            if (ok) ok = mbar_wait(&v_empty[st], free_parity, a.err);
-            if (lane == 0 && ok) mbar_arrive_expect_tx(&v_full[st], bytes);
-            ok = __all_sync(0xffffffffu, ok);
-            if (lane < boxes && ok)
-              for (int c = 0; c < Lay::PANELS; ++c)
-                tma_load_4d(dv + c * BN * 128 + lane * a.box * 128, &m_vc, c * 64, a.v_head_first ? p.h : off,
-                            a.v_head_first ? off : p.h, blk, &v_full[st]);
+            if (lane == 0) mbar_arrive_expect_tx(&full[st], uint32_t(boxes) * a.box * D * 2);
+            __syncwarp();
+            if (lane_box < boxes)
+              tma_load_4d(dst + lane_c * BN * 128 + lane_box * a.box * 128, m_c, lane_c * 64,
+                          c_head_first ? p.h : off, c_head_first ? off : p.h, blk, &full[st]);
           } else {
-            ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[st], free_parity, a.err));
-            if (ok) {
-              copy_paged_tile<D>(dk, reinterpret_cast<const uint16_t*>(a.kc), a.kc_b, a.kc_t, p.h * a.kc_h, table, a,
-                                 t0, valid, lane);
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&k_full[st]);
-              ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[st], free_parity, a.err));
-            }
-            if (ok) {
-              copy_paged_tile<D>(dv, reinterpret_cast<const uint16_t*>(a.vc), a.vc_b, a.vc_t, p.h * a.vc_h, table, a,
-                                 t0, valid, lane);
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&v_full[st]);
-            }
+            copy_paged_tile<D>(dst, reinterpret_cast<const uint16_t*>(is_v ? a.vc : a.kc), is_v ? a.vc_b : a.kc_b,
+                               is_v ? a.vc_t : a.kc_t, p.h * (is_v ? a.vc_h : a.kc_h), table, a, t0, valid, lane);
+            publish(&full[st]);
           }
         } else {
-          const int r0 = (j - p.s.nt_ctx) * BN, valid = min(BN, p.s.n - r0), row = p.s.lo + r0;
-          ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[st], free_parity, a.err));
+          const int r0 = (j - p.s.nt_ctx) * BN, row = p.s.lo + r0;
           if (a.tree_tma) {
-            if (ok && lane == 0) {
-              mbar_arrive_expect_tx(&k_full[st], Lay::TILE);
-              for (int c = 0; c < Lay::PANELS; ++c)
-                tma_load_3d(dk + c * BN * 128, &m_kt, c * 64, a.kt_head_first ? p.h : row,
-                            a.kt_head_first ? row : p.h, &k_full[st]);
-            }
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[st], free_parity, a.err));
-            if (ok && lane == 0) {
-              mbar_arrive_expect_tx(&v_full[st], Lay::TILE);
-              for (int c = 0; c < Lay::PANELS; ++c)
-                tma_load_3d(dv + c * BN * 128, &m_vt, c * 64, a.vt_head_first ? p.h : row,
-                            a.vt_head_first ? row : p.h, &v_full[st]);
-            }
+            if (lane == 0) mbar_arrive_expect_tx(&full[st], Lay::TILE);
+            __syncwarp();
+            if (lane < Lay::PANELS)
+              tma_load_3d(dst + lane * BN * 128, m_t, lane * 64, t_head_first ? p.h : row, t_head_first ? row : p.h,
+                          &full[st]);
           } else {
-            if (ok) {
-              copy_tile<D>(dk, reinterpret_cast<const uint16_t*>(a.kt) + row * a.kt_r + p.h * a.kt_h, a.kt_r, valid,
-                           lane);
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&k_full[st]);
-              ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[st], free_parity, a.err));
-            }
-            if (ok) {
-              copy_tile<D>(dv, reinterpret_cast<const uint16_t*>(a.vt) + row * a.vt_r + p.h * a.vt_h, a.vt_r, valid,
-                           lane);
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&v_full[st]);
-            }
+            const int64_t s_r = is_v ? a.vt_r : a.kt_r;
+            copy_tile<D>(dst, reinterpret_cast<const uint16_t*>(is_v ? a.vt : a.kt) + row * s_r +
+                                  p.h * (is_v ? a.vt_h : a.kt_h),
+                         s_r, min(BN, p.s.n - r0), lane);
+            publish(&full[st]);
           }
         }
+        ++g;
       }
     }
     // every issued copy lands before the CTA may exit
-    for (int i = max(0, g - ST); i < g; ++i) {
-      mbar_wait(&k_full[i % ST], (i / ST) & 1, nullptr);
-      mbar_wait(&v_full[i % ST], (i / ST) & 1, nullptr);
-    }
-  } else if (busy && warp == 5) {
-    // --------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t fmt = std::is_same<T, bf16>::value ? ~0u : ~((1u << 7) | (1u << 10));  // f16: type 0
-      constexpr uint32_t idesc_qk = idesc_bf16(BM, BN, false) & fmt;
-      constexpr uint32_t idesc_pv = idesc_bf16(BM, D, true) & fmt;
-      const uint32_t q0 = smem_u32(smem), k0 = smem_u32(smem + Lay::OFF_K), v0 = smem_u32(smem + Lay::OFF_V);
-      bool ok = true;
-      int g = 0, item = 0;
-      auto pv = [&](int gg, bool first) {
-        const int st = gg % ST;
-        ok = mbar_wait(&p_full[gg & 1], (gg >> 1) & 1, a.err) && mbar_wait(&v_full[st], (gg / ST) & 1, a.err);
-        if (!ok) return;
-        tc_fence_after();
-#pragma unroll
-        for (int kk = 0; kk < BN / 16; ++kk)
-          umma_f16_ta(tO, tmem + (gg & 1) * BN + kk * 8, smem_desc_sw128(v0 + st * Lay::TILE + kk * 2048, BN * 128, 1024),
-                      idesc_pv, (!first || kk > 0) ? 1u : 0u);
-        umma_commit(&v_empty[st]);
-        umma_commit(&pv_done[gg & 1]);
-      };
-      while (ok && walk.next(a, p)) {
-        ok = mbar_wait(q_full, item & 1, a.err);
-        for (int j = p.t0; j < p.t1 && ok; ++j, ++g) {
-          const int st = g % ST;
-          ok = mbar_wait(&k_full[st], (g / ST) & 1, a.err);
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            umma_f16(tmem + (g & 1) * BN, smem_desc_sw128(q0 + (kk >> 2) * BM * 128 + (kk & 3) * 32, 16, 1024),
-                     smem_desc_sw128(k0 + st * Lay::TILE + (kk >> 2) * BN * 128 + (kk & 3) * 32, 16, 1024), idesc_qk,
-                     kk > 0 ? 1u : 0u);
-          umma_commit(&s_full[g & 1]);
-          umma_commit(&k_empty[st]);
-          if (j > p.t0) pv(g - 1, j - 1 == p.t0);
+    for (int i = max(0, g - ST); i < g; ++i) mbar_wait(&full[i % ST], (i / ST) & 1, nullptr);
+    for (int i = max(0, qc - 2); i < qc; ++i) mbar_wait(&q_full[i & 1], (i >> 1) & 1, nullptr);
+  } else if (busy && warp >= 10) {
+    // -------------------------------------------------------- MMA issuers
+    // Warps 10 and 11 issue S = Q K^T of streams 0 and 1, warps 12 and 13
+    // issue O += P V.  Issue is the narrow place: the products of a unit take
+    // 640 cycles, but a wait that need not wait costs 100 and a commit 50 to
+    // 100; one warp for all needed 1430 cycles a unit, two needed 1100.
+    // The warps run their loops whole, on values that the compiler can see to
+    // be uniform (counts broadcast by shuffles, no early exits), so that the
+    // descriptors live in uniform registers: 29 cycles to issue an MMA; from a
+    // lane-0 branch it took 95 to 115.  After a wait that ran out, later
+    // waits are skipped and the loop ends.
+    constexpr uint32_t fmt = std::is_same<T, bf16>::value ? ~0u : ~((1u << 7) | (1u << 10));  // f16: type 0
+    constexpr uint32_t idesc_qk = idesc_bf16(BM, BN, false) & fmt;
+    constexpr uint32_t idesc_pv = idesc_bf16(BM, D, true) & fmt;
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const int role = __shfl_sync(0xffffffffu, warp, 0) - 10;
+    const int stream = role & 1;
+    bool alive = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      if (alive) alive = mbar_wait(bar, parity, a.err);
+      __syncwarp();
+    };
+    // A parity wait is right only for the phase after the last one that is
+    // known to be complete, and loads may complete out of order.  So both
+    // streams' issuers wait for every phase of every full barrier in order,
+    // also of tiles that only the other stream uses, and both arrive on the
+    // empty barriers (two arrivals): by commit after their products, plainly
+    // where they have none.
+    int g0 = 0, u0 = 0, qc = 0, item = 0;  // tiles, units, Q tiles, pieces before this one
+    const uint64_t dq0 = smem_desc_sw128(smem_u32(smem), 16, 1024);
+    const uint64_t dk0 = smem_desc_sw128(smem_u32(smem + Lay::OFF_K), 16, 1024);
+    const uint64_t dv0 = smem_desc_sw128(smem_u32(smem + Lay::OFF_V), BN * 128, 1024);
+    while (__shfl_sync(0xffffffffu, int(walk.next(a, p)), 0)) {
+      const int tiles = __shfl_sync(0xffffffffu, p.t1 - p.t0, 0);
+      const int two = __shfl_sync(0xffffffffu, int(p.two), 0);
+      const int k = two ? stream ^ (u0 & 1) : 0;
+      const int i0 = two ? 0 : (u0 & 1) ^ stream, di = 2 - two;
+      const bool idle = i0 >= tiles;  // a single tile, and the other stream has it
+      if (role < 2) {
+        const int qb = (qc + k) & 1;
+        for (int x = 0; x <= two; ++x) {
+          const int buf = (qc + x) & 1;
+          wait(&q_full[buf], ((qc + x) >> 1) & 1);
+          if ((idle || x != k) && elect_one()) mbar_arrive(&q_empty[buf]);
+          __syncwarp();
         }
-        if (ok) pv(g - 1, p.t1 - 1 == p.t0);
-        if (ok) umma_commit(o_full);
+        const uint64_t dq = dq0 + uint64_t(uint32_t(qb * Lay::Q_BYTES) >> 4);
+        for (int i = 0; i < tiles; ++i) {
+          const int g = g0 + i, st = g % ST;
+          wait(&k_full[st], (g / ST) & 1);
+          if (two || (i & 1) == i0) {
+            const int u = two ? u0 + 2 * i + k : u0 + i;
+            wait(&pv_done[u & 3], ((u >> 2) & 1) ^ 1);  // P(u - 4) has been read
+            tc_fence_after();
+            if (elect_one()) {
+              const uint64_t dk = dk0 + uint64_t(uint32_t(st * Lay::TILE) >> 4);
+#pragma unroll
+              for (int kk = 0; kk < D / 16; ++kk)
+                umma_f16(tm + (u & 3) * BN, dq + (((kk >> 2) * BM * 128 + (kk & 3) * 32) >> 4),
+                         dk + (((kk >> 2) * BN * 128 + (kk & 3) * 32) >> 4), idesc_qk, kk > 0 ? 1u : 0u);
+              umma_commit(&s_full[u & 3]);
+              umma_commit(&k_empty[st]);
+              if (i + di >= tiles) umma_commit(&q_empty[qb]);
+            }
+          } else if (elect_one()) {
+            mbar_arrive(&k_empty[st]);
+          }
+          __syncwarp();
+        }
+        qc += 1 + two;
+      } else {
+        // the first product of a piece overwrites O, which the rows of the
+        // piece before must have left
+        wait(o_empty, (item & 1) ^ 1);
+        for (int i = 0; i < tiles; ++i) {
+          const int g = g0 + i, st = g % ST;
+          wait(&v_full[st], (g / ST) & 1);
+          if (two || (i & 1) == i0) {
+            const int u = two ? u0 + 2 * i + k : u0 + i;
+            wait(&p_full[u & 3], (u >> 2) & 1);
+            tc_fence_after();
+            if (elect_one()) {
+              const uint64_t dv = dv0 + uint64_t(uint32_t(st * Lay::TILE) >> 4);
+              const uint32_t to = tm + 4 * BN + stream * 128, tp = tm + (u & 3) * BN;
+#pragma unroll
+              for (int kk = 0; kk < BN / 16; ++kk)
+                umma_f16_ta(to, tp + kk * 8, dv + kk * (2048 >> 4), idesc_pv, (i != i0 || kk > 0) ? 1u : 0u);
+              umma_commit(&pv_done[u & 3]);
+              umma_commit(&v_empty[st]);
+              if (i + di >= tiles) umma_commit(o_full);
+            }
+          } else if (elect_one()) {
+            mbar_arrive(&v_empty[st]);
+          }
+          __syncwarp();
+        }
+        if (idle && elect_one()) mbar_arrive(o_full);
+        __syncwarp();
         ++item;
       }
+      g0 += tiles;
+      u0 += tiles * (1 + two);
     }
+    // every product and every arrival of this warp is done before the CTA
+    // gives its memory back
+    if (elect_one()) umma_commit(&drain[role]);
+    __syncwarp();
+    mbar_wait(&drain[role], 0, nullptr);
   } else if (busy) {
     // ------------------------------------------------------------ softmax
-    const int row = threadIdx.x;
-    const uint32_t lane_off = uint32_t(warp * 32) << 16;
+    const int stream = warp >> 2;
+    const int row = threadIdx.x & 127;
+    const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t tOs = tO + stream * 128 + lane_off;
     const float sl2 = a.scale_log2;
     bool ok = true;
-    int g = 0, item = 0;
+    int g = 0, u0 = 0, item = 0;  // tiles and units before the piece, pieces
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      ok = ok && mbar_wait(bar, parity, a.err);
+      ok = __all_sync(0xffffffffu, ok);
+    };
     while (walk.next(a, p)) {
-      const int rows = p.s.n * a.group - p.mi * BM;  // valid rows of the tile (may exceed it)
-      // Q rows: the previous piece's last S tile has been seen, so its Q is free
-      {
-        const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q);
-        constexpr int C = D / 8;
-        const int most = min(rows, BM);
-        for (int e = threadIdx.x; e < most * C; e += 128) {
-          const int r = e / C, c = e % C, flat = p.mi * BM + r, node = flat / a.group, hg = flat % a.group;
-          const uint4 v = *reinterpret_cast<const uint4*>(q + int64_t(p.s.lo + node) * a.q_r +
-                                                          int64_t(p.h * a.group + hg) * a.q_h + c * 8);
-          *reinterpret_cast<uint4*>(smem + tile_offset(BM, r, c)) = v;
-        }
-        fence_proxy_async_smem();
-        mbar_arrive(q_full);
-      }
-      const bool live = warp * 32 < rows;  // warps without a valid row only keep the barriers going
-      const int flat = p.mi * BM + row, node = flat / a.group;
+      const int tiles = p.t1 - p.t0;
+      const int k = p.two ? stream ^ (u0 & 1) : 0;  // this stream's row tile
+      const int rows = p.rows(a, k);
+      const bool live = (warp & 3) * 32 < rows;  // warps without a valid row only keep the barriers going
+      const int node = (2 * p.pair + k) * a.nodes + row / a.group;
       const bool mine = row < rows;
       float m_ref = -INFINITY, l0 = 0.f, l1 = 0.f;
-      bool odd = false;  // the piece's tree V holds values that are not finite
-      for (int j = p.t0; j < p.t1; ++j, ++g) {
-        const int buf = g & 1, st = g % ST;
+      bool odd = false;   // the piece's tree V holds values that are not finite
+      bool fresh = true;  // no unit of this stream yet
+      const int i0 = p.two ? 0 : (u0 & 1) ^ stream, di = p.two ? 1 : 2;
+      for (int i = i0; i < tiles; i += di) {
+        const int j = p.t0 + i, u = p.two ? u0 + 2 * i + k : u0 + i;
+        const int buf = u & 3, st = (g + i) % ST;
         const uint32_t tS = tmem + buf * BN + lane_off;
         const bool tree = j >= p.s.nt_ctx;
         const int col0 = tree ? (j - p.s.nt_ctx) * BN : j * BN;
         const int valid = min(BN, (tree ? p.s.n : p.s.ctx) - col0);
-        ok = ok && mbar_wait(&s_full[buf], (g >> 1) & 1, a.err);
-        ok = __all_sync(0xffffffffu, ok);
+        wait(&s_full[buf], (u >> 2) & 1);
         tc_fence_after();
         if (tree || valid < BN) {
           // P is zero in masked places, but zero times an infinity or NaN is
           // not: rows past the end are cleared, and values of tree rows that
           // are not finite are cleared here and added back to the rows that
-          // see them after the last product.
-          ok = ok && mbar_wait(&v_full[st], (g / ST) & 1, a.err);
-          ok = __all_sync(0xffffffffu, ok);
+          // see them after the last product.  (The stage's phase before this
+          // one is complete: S(u) came after P V of unit u - 4, at most four
+          // tiles back, whose issuer had waited for every tile before it.)
+          wait(&v_full[st], ((g + i) / ST) & 1);
+          const int tag = p.two ? u0 + 2 * i : u;
+          const int part = p.two ? threadIdx.x : row, parts = p.two ? 256 : 128;
           if (ok) {
-            const int r = row >> 1, part = row & 1;
-            constexpr int HC = D / 16;  // 16-byte chunks of half a row
             uint8_t* v = smem + Lay::OFF_V + st * Lay::TILE;
-            if (r >= valid) {
-              for (int c = 0; c < HC; ++c)
-                *reinterpret_cast<uint4*>(v + tile_offset(BN, r, part * HC + c)) = make_uint4(0, 0, 0, 0);
-            } else if (tree) {
-              for (int c = 0; c < HC; ++c) {
-                uint32_t* w = reinterpret_cast<uint32_t*>(v + tile_offset(BN, r, part * HC + c));
-                for (int e = 0; e < 4; ++e)
-                  if (odd2<T>(w[e])) {
-                    uint16_t* h = reinterpret_cast<uint16_t*>(w + e);
-                    if (odd2<T>(h[0])) h[0] = 0;
-                    if (odd2<T>(h[1])) h[1] = 0;
-                    s_odd[buf] = uint32_t(g) + 1;
-                  }
+            for (int e = part; e < BN * (D / 8); e += parts) {
+              const int r = e / (D / 8);
+              uint4* w = reinterpret_cast<uint4*>(v + tile_offset(BN, r, e % (D / 8)));
+              if (r >= valid) {
+                *w = make_uint4(0, 0, 0, 0);
+              } else if (tree) {
+                const uint4 x = *w;
+                if (odd2<T>(x.x) || odd2<T>(x.y) || odd2<T>(x.z) || odd2<T>(x.w)) {
+                  uint16_t* h = reinterpret_cast<uint16_t*>(w);
+                  for (int c = 0; c < 8; ++c)
+                    if (odd2<T>(h[c])) h[c] = 0;
+                  sh.odd[tag & 3] = uint32_t(tag) + 1;
+                }
               }
             }
             fence_proxy_async_smem();
           }
-          softmax_sync();
-          if (tree) odd = odd || s_odd[buf] == uint32_t(g) + 1;
+          __syncwarp();  // bar.sync and the tcgen05 loads and stores want whole warps
+          bar_sync(p.two ? 3 : 1 + stream, parts);
+          if (tree) odd = odd || sh.odd[tag & 3] == uint32_t(tag) + 1;
         }
         if (live && ok) {
           uint32_t r[2][32];
@@ -564,6 +689,7 @@ __global__ void __launch_bounds__(kThreads, 2)
               }
               vis[w] = in;
             }
+            __syncwarp();
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -572,7 +698,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
           float mxa[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mxa[i] = -INFINITY;
+          for (int x = 0; x < 4; ++x) mxa[x] = -INFINITY;
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -585,6 +711,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           const float m_use = rescale ? mxs : m_ref;
           const float neg_m = m_use == -INFINITY ? 0.f : -m_use;  // nothing visible yet: all P are 0
           float sa[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+          __syncwarp();
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             uint32_t pk[16];
@@ -599,19 +726,19 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
             tmem_st16(tS + c * 16, pk);
           }
-          if (__any_sync(0xffffffffu, rescale && j > p.t0)) {
-            ok = mbar_wait(&pv_done[buf ^ 1], ((g - 1) >> 1) & 1, a.err);
-            ok = __all_sync(0xffffffffu, ok);
+          if (!fresh && __any_sync(0xffffffffu, rescale)) {
+            wait(&pv_done[(u - 2) & 3], ((u - 2) >> 2) & 1);
             tc_fence_after();
             const float f = rescale ? ex2(m_ref - m_use) : 1.0f;
+            __syncwarp();
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               uint32_t o[32];
-              tmem_ld32(tO + lane_off + c * 32, o);
+              tmem_ld32(tOs + c * 32, o);
               tmem_wait_ld();
 #pragma unroll
               for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tmem_st32(tO + lane_off + c * 32, o);
+              tmem_st32(tOs + c * 32, o);
             }
             l0 *= f;
             l1 *= f;
@@ -621,67 +748,111 @@ __global__ void __launch_bounds__(kThreads, 2)
           l0 += sa[0][0] + sa[1][0];
           l1 += sa[0][1] + sa[1][1];
         }
+        fresh = false;
         tc_fence_before();
         __syncwarp();
         if (lane == 0 && ok) mbar_arrive(&p_full[buf]);
       }
       // the piece's O is complete
-      ok = ok && mbar_wait(o_full, item & 1, a.err);
-      ok = __all_sync(0xffffffffu, ok);
-      ++item;
-      if (!ok || !live) continue;
+      wait(o_full, item & 1);
       tc_fence_after();
-      const float l = l0 + l1;
-      const int64_t slot = 2 * int64_t(blockIdx.x) + (p.starts ? 1 : 0);
-      const float inv = p.whole ? (l > 0.f || l != l ? 1.0f / l : 0.f) : 1.0f;
-      const int qh = p.h * a.group + flat % a.group;
-      uint16_t* orow = reinterpret_cast<uint16_t*>(a.out) + int64_t(p.s.lo + node) * a.out_r + int64_t(qh) * a.out_h;
-      float* prow = a.part_o + (slot * a.part_rows + row) * D;
+      float l = l0 + l1, f0 = 1.f, f1 = 0.f, m = m_ref;
+      const bool join = !p.two && tiles > 1;  // both streams hold a part of every row
+      if (!p.two) {
+        sh.ml[stream][row] = make_float2(m_ref, l);
+        if (row == 0) sh.piece_odd[stream] = odd;
+        __syncwarp();
+        bar_sync(4, 256);
+        const float2 x = sh.ml[0][row], y = sh.ml[1][row];
+        m = fmaxf(x.x, y.x);
+        // weights of the two streams; the one without a unit is not read
+        const int only = u0 & 1;
+        f0 = join || only == 0 ? (x.x == -INFINITY ? 0.f : ex2(x.x - m)) : 0.f;
+        f1 = join || only == 1 ? (y.x == -INFINITY ? 0.f : ex2(y.x - m)) : 0.f;
+        l = x.y * f0 + y.y * f1;
+        odd = sh.piece_odd[0] || sh.piece_odd[1];
+      }
+      if (ok && live) {
+        const int64_t rec =
+            ((2 * int64_t(blockIdx.x) + (p.starts ? 1 : 0)) * 2 + k) * a.part_rows + row;
+        const float inv = p.whole ? (l > 0.f || l != l ? 1.0f / l : 0.f) : 1.0f;
+        const int qh = p.h * a.group + row % a.group;
+        uint16_t* orow = reinterpret_cast<uint16_t*>(a.out) + int64_t(p.s.lo + node) * a.out_r + int64_t(qh) * a.out_h;
+        float* prow = a.part_o + rec * D;
+        // two row tiles: all columns of the own one; else half of the columns of both streams' O
+        constexpr int NC = D / 32;
+        const int c_lo = p.two ? 0 : stream * (NC / 2), c_hi = p.two ? NC : c_lo + NC / 2;
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld32(tO + lane_off + c * 32, o);
-        tmem_wait_ld();
-        if (mine && odd) {
-          const int from = max(p.t0 - p.s.nt_ctx, 0) * BN, upto = min((p.t1 - p.s.nt_ctx) * BN, p.s.n);
-          for (int t = from; t < upto; ++t) {
-            const bool sees = a.mask == nullptr
-                                  ? t <= node
-                                  : (t >> 5) < a.words &&
-                                        (uint32_t(a.mask[int64_t(p.s.lo + node) * a.words + (t >> 5)]) >> (t & 31)) & 1u;
-            if (!sees) continue;
-            const T* v = reinterpret_cast<const T*>(a.vt) + int64_t(p.s.lo + t) * a.vt_r + p.h * a.vt_h + c * 32;
+        for (int c = c_lo; c < c_hi; ++c) {
+          uint32_t o[32];
+          __syncwarp();
+          if (p.two) {
+            tmem_ld32(tOs + c * 32, o);
+            tmem_wait_ld();
+          } else {
+            tmem_ld32(tO + ((u0 & 1) ? 128 : 0) + lane_off + c * 32, o);
+            if (join) {
+              uint32_t o2[32];
+              tmem_ld32(tO + ((u0 & 1) ? 0 : 128) + lane_off + c * 32, o2);
+              tmem_wait_ld();
+              const float fa = (u0 & 1) ? f1 : f0, fb = (u0 & 1) ? f0 : f1;
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const float x = as_float<T>(v[e]);
-              if (!(fabsf(x) < INFINITY)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
+              for (int e = 0; e < 32; ++e)
+                o[e] = __float_as_uint(fmaf(__uint_as_float(o[e]), fa, __uint_as_float(o2[e]) * fb));
+            } else {
+              tmem_wait_ld();
             }
           }
-        }
-        if (mine && p.whole) {
+          if (mine && odd) {
+            const int from = max(p.t0 - p.s.nt_ctx, 0) * BN, upto = min((p.t1 - p.s.nt_ctx) * BN, p.s.n);
+            for (int t = from; t < upto; ++t) {
+              const bool sees =
+                  a.mask == nullptr
+                      ? t <= node
+                      : (t >> 5) < a.words &&
+                            (uint32_t(a.mask[int64_t(p.s.lo + node) * a.words + (t >> 5)]) >> (t & 31)) & 1u;
+              if (!sees) continue;
+              const T* v = reinterpret_cast<const T*>(a.vt) + int64_t(p.s.lo + t) * a.vt_r + p.h * a.vt_h + c * 32;
 #pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            uint4 w;
-            w.x = pack2<T>(__uint_as_float(o[8 * v + 0]) * inv, __uint_as_float(o[8 * v + 1]) * inv);
-            w.y = pack2<T>(__uint_as_float(o[8 * v + 2]) * inv, __uint_as_float(o[8 * v + 3]) * inv);
-            w.z = pack2<T>(__uint_as_float(o[8 * v + 4]) * inv, __uint_as_float(o[8 * v + 5]) * inv);
-            w.w = pack2<T>(__uint_as_float(o[8 * v + 6]) * inv, __uint_as_float(o[8 * v + 7]) * inv);
-            *reinterpret_cast<uint4*>(orow + c * 32 + v * 8) = w;
+              for (int e = 0; e < 32; ++e) {
+                const float x = as_float<T>(v[e]);
+                if (!(fabsf(x) < INFINITY)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
+              }
+            }
           }
-        } else if (mine) {
+          if (mine && p.whole) {
 #pragma unroll
-          for (int v = 0; v < 8; ++v)
-            *reinterpret_cast<uint4*>(prow + c * 32 + v * 4) =
-                make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+            for (int v = 0; v < 4; ++v) {
+              uint4 w;
+              w.x = pack2<T>(__uint_as_float(o[8 * v + 0]) * inv, __uint_as_float(o[8 * v + 1]) * inv);
+              w.y = pack2<T>(__uint_as_float(o[8 * v + 2]) * inv, __uint_as_float(o[8 * v + 3]) * inv);
+              w.z = pack2<T>(__uint_as_float(o[8 * v + 4]) * inv, __uint_as_float(o[8 * v + 5]) * inv);
+              w.w = pack2<T>(__uint_as_float(o[8 * v + 6]) * inv, __uint_as_float(o[8 * v + 7]) * inv);
+              *reinterpret_cast<uint4*>(orow + c * 32 + v * 8) = w;
+            }
+          } else if (mine) {
+#pragma unroll
+            for (int v = 0; v < 8; ++v)
+              *reinterpret_cast<uint4*>(prow + c * 32 + v * 4) =
+                  make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+          }
         }
+        if (mine && !p.whole && (p.two || stream == 0)) a.part_ml[rec] = make_float2(m, l);
       }
-      if (mine && !p.whole) a.part_ml[slot * a.part_rows + row] = make_float2(m_ref, l);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0 && ok) mbar_arrive(o_empty);
+      ++item;
+      g += tiles;
+      u0 += tiles * (p.two ? 2 : 1);
     }
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == 9) {
     tc_fence_after();
+    __syncwarp();
     tmem_dealloc<Lay::TMEM_COLS>(tmem);
   }
 }
@@ -717,31 +888,66 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs a) {
     return;
   }
   const int64_t share = a.base[a.B];
-  const int h = qh / a.group, flat = (r - s.lo) * a.group + qh % a.group, mi = flat / BM, row = flat % BM;
+  const int h = qh / a.group, node = r - s.lo, mi = node / a.nodes, pair = mi >> 1;
+  const int row = (node % a.nodes) * a.group + qh % a.group;
+  if (share <= 0) return;
   const Segments seg(s, share);
-  const int64_t first = a.base[b] + int64_t(h) * s.mt * s.nt;
+  const int64_t first = a.base[b] + int64_t(h) * s.pairs * s.nt;
+  auto segment_first = [&](int i) { return first + int64_t(seg.start(i)) * s.pairs + int64_t(pair) * seg.length(i); };
+  // Records by number: a segment of an item with several is at most twice a
+  // share long, so it touches up to three CTAs, four numbers each; a single
+  // segment has one for each of its CTAs.
+  const int64_t begin = segment_first(0), end = begin + seg.length(0) - 1;
+  const int width = seg.count == 1 ? int(end / share - begin / share) + 1 : 4;
+  if (seg.count == 1 && width == 1) return;  // one CTA had the whole item
   float m = -INFINITY, l = 0.f;
-  for (int i = 0; i < seg.count; ++i) {
-    const int64_t g0 = first + int64_t(seg.start(i)) * s.mt + int64_t(mi) * seg.length(i);
-    const int64_t c0 = g0 / share, c1 = (g0 + seg.length(i) - 1) / share;
-    if (seg.count == 1 && c0 == c1) return;  // one CTA had the whole item
-    for (int64_t c = c0; c <= c1; ++c) {
-      const int64_t rec = (2 * c + (c == c0 ? 1 : 0)) * a.part_rows + row;
-      const float2 ml = a.part_ml[rec];
-      float o[E];
-      const float* po = a.part_o + rec * D + lane * E;
-      if constexpr (E == 4) *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(po);
-      else *reinterpret_cast<float2*>(o) = *reinterpret_cast<const float2*>(po);
-      const float mx = fmaxf(m, ml.x);
-      if (mx == -INFINITY) {  // nothing visible so far; a NaN sum still counts
-        l += ml.y;
-        continue;
+  for (int k0 = 0; k0 < seg.count * width; k0 += 32) {
+    // every lane takes one record's maximum and sum
+    const int k = k0 + lane, i = k / width;
+    int64_t rec = -1;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (i < seg.count) {
+      const int64_t g0 = segment_first(i), c0 = g0 / share, c = c0 + k % width;
+      if (c <= (g0 + seg.length(i) - 1) / share && c >= 0 && c < a.ctas) {
+        rec = ((2 * c + (c == c0 ? 1 : 0)) * 2 + (mi & 1)) * a.part_rows + row;
+        ml = a.part_ml[rec];
       }
-      const float f = ex2(m - mx), k = ex2(ml.x - mx);
-      l = l * f + ml.y * k;
+    }
+    float mx = fmaxf(m, ml.x);
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = acc[e] * f + (ml.x == -INFINITY ? 0.f : o[e] * k);
-      m = mx;
+    for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+    const float f = m == -INFINITY ? 0.f : ex2(m - mx);
+    const float weight = ml.x == -INFINITY ? 0.f : ex2(ml.x - mx);
+    float ls = ml.y * weight;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, d);
+    l = l * f + ls;
+    m = mx;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] *= f;
+    // the records' rows in order, four loads in flight
+    uint32_t todo = __ballot_sync(0xffffffffu, rec >= 0);
+    while (todo) {
+      float o[4][E], w[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int from = todo ? __ffs(todo) - 1 : 0;
+        const int64_t at = __shfl_sync(0xffffffffu, rec, from);
+        w[x] = __shfl_sync(0xffffffffu, weight, from);
+        if (!todo) w[x] = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[x][e] = 0.f;
+        if (todo) {
+          const float* po = a.part_o + at * D + lane * E;
+          if constexpr (E == 4) *reinterpret_cast<float4*>(o[x]) = *reinterpret_cast<const float4*>(po);
+          else *reinterpret_cast<float2*>(o[x]) = *reinterpret_cast<const float2*>(po);
+        }
+        todo &= todo - 1;
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(o[x][e], w[x], acc[e]);
     }
   }
   const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
@@ -768,7 +974,7 @@ EncodeFn encode_fn() {
 
 // `t` [..., rows, heads, D] (3-D) or [blocks, rows, heads, D] (4-D); false if
 // the layout does not fit a tensor map.
-bool encode_rows(CUtensorMap& m, const torch::Tensor& t, int box_rows, bool& head_first) {
+bool encode_rows(CUtensorMap& m, const torch::Tensor& t, int box_rows, bool& head_first, int box_heads = 1) {
   const int rank = int(t.dim());
   const int64_t rows = t.size(rank - 3), heads = t.size(rank - 2);
   const int64_t s_row = t.stride(rank - 3) * 2, s_head = t.stride(rank - 2) * 2;
@@ -790,6 +996,7 @@ bool encode_rows(CUtensorMap& m, const torch::Tensor& t, int box_rows, bool& hea
   for (int d = 0; d + 1 < rank; ++d)
     if (strides[d] < row_bytes || strides[d] % 16 != 0 || strides[d] >= (cuuint64_t(1) << 40)) return false;
   box[dr] = cuuint32_t(box_rows);
+  box[dh] = cuuint32_t(box_heads);
   return encode_fn()(&m,
                      t.scalar_type() == at::kHalf ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                      cuuint32_t(rank), t.data_ptr(), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -802,7 +1009,7 @@ void launch(const CUtensorMap* m, const TreeArgs& a, int grid, cudaStream_t st) 
   // per device, so set at every launch (a few hundred nanoseconds)
   KVS_CUDA_CHECK(cudaFuncSetAttribute(tree_attention_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       Layout<D>::SMEM));
-  tree_attention_kernel<T, D><<<grid, kThreads, Layout<D>::SMEM, st>>>(m[0], m[1], m[2], m[3], a);
+  tree_attention_kernel<T, D><<<grid, kThreads, Layout<D>::SMEM, st>>>(m[0], m[1], m[2], m[3], m[4], a);
   KVS_CUDA_CHECK(cudaGetLastError());
   const int64_t warps = int64_t(a.R) * a.hkv * a.group;
   launch_pdl(tree_merge_kernel<T, D>, dim3(unsigned((warps + 3) / 4)), dim3(128), 0, st, a);
@@ -851,6 +1058,7 @@ void paged_tree_attention(torch::Tensor q, torch::Tensor k_tree, torch::Tensor v
     a.mask = tree_mask->data_ptr<int32_t>();
     a.words = int(tree_mask->size(1));
   }
+  KVS_CHECK_ARG(Hq / Hkv <= BM, "tree attention: at most 128 query heads per KV head");
   KVS_CHECK_ARG(scale > 0, "tree attention: scale must be positive");
   KVS_CHECK_ARG(R * Hq < (int64_t(1) << 30) && k_cache.size(1) >= 1 && k_cache.size(0) >= 1 &&
                     k_cache.size(0) <= INT32_MAX && k_cache.size(1) <= INT32_MAX,
@@ -893,15 +1101,22 @@ void paged_tree_attention(torch::Tensor q, torch::Tensor k_tree, torch::Tensor v
   a.err = reinterpret_cast<uint32_t*>(status.data_ptr<int32_t>());
   // TMA boxes of the cache: the largest power of two of at least 8 tokens that
   // tiles both a block and a K/V tile; other block sizes are copied
-  CUtensorMap m[4] = {};
+  CUtensorMap m[5] = {};
   const int box = std::min(BN, a.bs & -a.bs);
   a.box = box >= 8 && encode_rows(m[0], k_cache, box, a.k_head_first) && encode_rows(m[1], v_cache, box, a.v_head_first)
               ? box
               : 0;
   a.tree_tma = encode_rows(m[2], k_tree, BN, a.kt_head_first) && encode_rows(m[3], v_tree, BN, a.vt_head_first);
-  const int grid = 2 * at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  // Row tiles end at a tree node, and q boxes of 8 nodes (one box for large
+  // groups) keep every box at the start of a swizzle pattern.
+  a.q_box = a.group <= 16 ? 8 : BM / a.group;
+  a.nodes = BM / a.group / a.q_box * a.q_box;
+  bool q_head_first = false;
+  a.q_tma = encode_rows(m[4], q, a.q_box, q_head_first, a.group) && q_head_first;
+  const int grid = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   a.part_rows = int(std::min<int64_t>(BM, R * a.group));
-  const int64_t recs = int64_t(2) * grid * a.part_rows;
+  a.ctas = grid;
+  const int64_t recs = int64_t(4) * grid * a.part_rows;
   torch::Tensor scratch = torch::empty({recs * (D + 2) + 2 * (B + 1)}, q.options().dtype(at::kFloat));
   a.part_o = scratch.data_ptr<float>();
   a.part_ml = reinterpret_cast<float2*>(a.part_o + recs * D);

@@ -52,9 +52,9 @@ struct TreeArgs {
   int ctas;
   int part_rows;   // rows kept per partial record
   float scale_log2;
-  float* part_o;    // [4 * CTAs, part_rows, D]
+  float4* part_o;   // [4 * CTAs, D / 4, part_rows]: neighbouring lanes write neighbouring rows
   float2* part_ml;  // [4 * CTAs, part_rows]
-  int64_t* base;    // [B + 1] first tile of each request, then the share
+  int4* meta;       // [CTAs] request of the CTA's first tile, that request's first tile, share, total
   uint32_t* err;
 };
 
@@ -82,10 +82,15 @@ __device__ __forceinline__ int64_t tile_count(const TreeArgs& a, const Shape& s)
 // but the first find it in L2.
 struct Segments {
   int count, len, longer;  // `longer` segments of len + 1 tiles, then segments of len
-  __device__ __forceinline__ Segments(const Shape& s, int64_t share) {
-    count = s.pairs > 1 ? int(max(int64_t(1), int64_t(s.nt) / share)) : 1;
-    len = s.nt / count;
-    longer = s.nt % count;
+  __device__ __forceinline__ Segments(const Shape& s, int share) {
+    count = 1;
+    len = s.nt;
+    longer = 0;
+    if (s.pairs > 1 && s.nt > share) {
+      count = s.nt / share;
+      len = s.nt / count;
+      longer = s.nt - len * count;
+    }
   }
   __device__ __forceinline__ int length(int i) const { return len + (i < longer ? 1 : 0); }
   __device__ __forceinline__ int start(int i) const { return i * len + min(i, longer); }
@@ -94,46 +99,53 @@ struct Segments {
 struct Piece {  // consecutive tiles of one item (request, KV head, pair of row tiles)
   Shape s;
   int b, h, pair;
-  int t0, t1;     // tiles [t0, t1) of the item
-  bool starts;    // begins its segment
-  bool whole;     // the complete item
-  bool two;       // the pair has two row tiles: each stream takes one; else the streams take turns in tiles
+  int segment, offset;  // of its first tile
+  int t0, t1;           // tiles [t0, t1) of the item
+  __device__ __forceinline__ bool starts() const { return offset == 0; }  // begins its segment
+  __device__ __forceinline__ bool whole() const { return t1 - t0 == s.nt; }
+  // the pair has two row tiles: each stream takes one; else the streams take turns in tiles
+  __device__ __forceinline__ bool two() const { return 2 * pair + 1 < s.mt; }
   __device__ __forceinline__ int rows(const TreeArgs& a, int k) const {
     return min(s.n - (2 * pair + k) * a.nodes, a.nodes) * a.group;
   }
 };
 
+// The item, segment and tile that the tile with number x of a request is.
+__device__ __forceinline__ void locate(const Shape& s, const Segments& seg, int x, Piece& p) {
+  const int per_head = s.pairs * s.nt;
+  p.h = x / per_head;
+  int y = x - p.h * per_head;
+  p.segment = p.pair = 0;
+  if (s.pairs > 1) {
+    const int big = (seg.len + 1) * s.pairs;
+    if (y < big * seg.longer) {
+      p.segment = y / big;
+    } else if (seg.count > 1) {
+      p.segment = seg.longer + (y - big * seg.longer) / (seg.len * s.pairs);
+    }
+    y -= seg.start(p.segment) * s.pairs;
+    p.pair = y / seg.length(p.segment);
+    y -= p.pair * seg.length(p.segment);
+  }
+  p.offset = y;
+  p.t0 = seg.start(p.segment) + y;
+}
+
 struct Walker {  // the pieces of one CTA's share, in order
-  int64_t at, end, base, share;
-  int b;
+  int at, end, base, share, b;
   Shape s;
   __device__ __forceinline__ bool next(const TreeArgs& a, Piece& p) {
     if (at >= end) return false;
-    while (at >= base + tile_count(a, s)) {
-      base += tile_count(a, s);
+    while (at >= base + int(tile_count(a, s))) {
+      base += int(tile_count(a, s));
       s = request_shape(a, ++b);
     }
     const Segments seg(s, share);
-    const int64_t x = at - base;
-    const int64_t per_head = int64_t(s.pairs) * s.nt;
     p.s = s;
     p.b = b;
-    p.h = int(x / per_head);
-    const int64_t y = x - p.h * per_head;
-    const int64_t big = int64_t(seg.len + 1) * s.pairs;
-    int i;
-    if (y < big * seg.longer) i = int(y / big);
-    else i = seg.longer + int((y - big * seg.longer) / (int64_t(seg.len) * s.pairs));
-    const int64_t z = y - int64_t(seg.start(i)) * s.pairs;
-    const int len = seg.length(i);
-    p.pair = int(z / len);
-    const int off = int(z - int64_t(p.pair) * len);
-    const int take = int(min(int64_t(len - off), end - at));
-    p.t0 = seg.start(i) + off;
+    locate(s, seg, at - base, p);
+    const int take = min(seg.length(p.segment) - p.offset, end - at);
     p.t1 = p.t0 + take;
-    p.starts = off == 0;
-    p.whole = take == s.nt;
-    p.two = 2 * p.pair + 1 < s.mt;
     at += take;
     return true;
   }
@@ -228,8 +240,8 @@ __device__ __forceinline__ uint32_t tile_offset(int rows, int r, int c) {
 
 struct Shared {
   float2 ml[2][BM];       // row maximum and sum of the two streams
-  int64_t sum[kThreads / 32], base;
-  int b;
+  int64_t sum[kThreads / 32];
+  int base, b;
   uint32_t tmem;
   uint32_t odd[4];        // 1 + the last unit whose tree V held values that are not finite
   uint32_t piece_odd[2];  // ... in the streams' tiles of the piece
@@ -312,24 +324,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_trigger();
 
-  if (threadIdx.x == 0) {
-    tma_prefetch_desc(&m_kc);
-    tma_prefetch_desc(&m_vc);
-    tma_prefetch_desc(&m_kt);
-    tma_prefetch_desc(&m_vt);
-    tma_prefetch_desc(&m_q);
-    for (int i = 0; i < Lay::NUM_BARS; ++i) {
-      uint64_t* bar = bars + i;
-      uint32_t arrivals = 1;
-      if ((bar >= k_empty && bar < k_empty + ST) || (bar >= v_empty && bar < v_empty + ST) ||
-          (bar >= q_empty && bar < q_empty + 2) || bar == o_full)
-        arrivals = 2;  // one for each stream
-      if (bar >= p_full && bar < p_full + 4) arrivals = 4;  // the warps of a stream
-      if (bar == o_empty) arrivals = 8;
-      mbar_init(bar, arrivals);
-    }
+  if (threadIdx.x < Lay::NUM_BARS) {
+    const int i = threadIdx.x, sb = i - 4 * ST;  // position after the ring's barriers
+    uint32_t arrivals = 1;
+    if ((i >= ST && i < 2 * ST) || (i >= 3 * ST && i < 4 * ST)) arrivals = 2;  // k_empty, v_empty: both streams
+    if (sb >= 4 && sb < 8) arrivals = 4;       // p_full: the warps of a stream
+    if (sb >= 14 && sb < 17) arrivals = 2;     // q_empty, o_full: both streams
+    if (sb == 17) arrivals = 8;                // o_empty: all softmax warps
+    mbar_init(&bars[i], arrivals);
     fence_barrier_init();
-    for (int i = 0; i < 4; ++i) sh.odd[i] = 0;
+  } else if (threadIdx.x < 64 + 5) {
+    if (threadIdx.x >= 64) {
+      const int i = threadIdx.x - 64;
+      tma_prefetch_desc(i == 0 ? &m_kc : i == 1 ? &m_vc : i == 2 ? &m_kt : i == 3 ? &m_vt : &m_q);
+    }
+  } else if (threadIdx.x >= 96 && threadIdx.x < 100) {
+    sh.odd[threadIdx.x - 96] = 0;
   }
   if (warp == 9) tmem_alloc<Lay::TMEM_COLS>(&sh.tmem);
 
@@ -337,21 +347,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   // find the request that this CTA's share begins in; a second pass is needed
   // only where the requests outnumber the threads.
   Walker walk;
-  walk.share = 0;
+  walk.share = 1;
+  walk.at = walk.end = 0;
   for (int pass = 0; pass < 2; ++pass) {
-    int64_t carry = 0, from = 0, mine = 0;
+    int64_t carry = 0;
+    int from = 0, mine = 0;
     auto settle = [&](int b) {
-      if (b >= a.B) return;
-      if (blockIdx.x == 0) a.base[b] = from;
-      if (walk.at >= from && walk.at < from + mine) {
+      if (b < a.B && walk.at >= from && walk.at - from < mine) {
         sh.b = b;
         sh.base = from;
       }
     };
     for (int b0 = 0; b0 < a.B; b0 += kThreads) {
       const int b = b0 + threadIdx.x;
-      mine = b < a.B ? tile_count(a, request_shape(a, b)) : 0;
-      int64_t x = mine;
+      const int64_t count = b < a.B ? tile_count(a, request_shape(a, b)) : 0;
+      int64_t x = count;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
@@ -360,25 +370,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncthreads();
       if (lane == 31) sh.sum[warp] = x;
       __syncthreads();
-      from = carry + x - mine;
+      int64_t before = carry + x - count;
 #pragma unroll
       for (int w = 0; w < kThreads / 32; ++w) {
-        from += w < warp ? sh.sum[w] : 0;
+        before += w < warp ? sh.sum[w] : 0;
         carry += sh.sum[w];
       }
+      from = int(before);
+      mine = int(count);
       if (pass == 1) settle(b);
     }
     if (pass == 0) {
-      walk.share = max((carry + gridDim.x - 1) / int64_t(gridDim.x), int64_t(a.min_share));
-      walk.at = blockIdx.x * walk.share;
-      walk.end = min(walk.at + walk.share, carry);
+      if (carry > INT32_MAX - 4096) {  // numbers of tiles are 32 bits; nothing is computed
+        if (threadIdx.x == 0) atomicCAS(a.err, 0u, uint32_t(kStatusBadSize));
+        carry = 0;
+        mine = 0;
+      }
+      const int total = int(carry);
+      walk.share = max((total + int(gridDim.x) - 1) / int(gridDim.x), a.min_share);
+      walk.at = int(min(int64_t(blockIdx.x) * walk.share, int64_t(total)));
+      walk.end = min(walk.at + walk.share, total);
       if (a.B <= kThreads) {
         settle(threadIdx.x);
         break;
       }
     }
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) a.base[a.B] = walk.share;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -390,6 +407,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     walk.base = sh.base;
     walk.s = request_shape(a, walk.b);
   }
+  if (threadIdx.x == 0)
+    a.meta[blockIdx.x] = busy ? make_int4(walk.b, walk.base, walk.share, 1) : make_int4(0, 0, 1, 0);
   Piece p;
 
   if (busy && (warp == 8 || warp == 9)) {
@@ -419,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     while (ok && walk.next(a, p)) {
       const int32_t* table = a.tables + p.b * a.table_stride;
       // block and offset of this lane's box in tile j
-      auto locate = [&](int j, int& blk, int& off) {
+      auto block_of = [&](int j, int& blk, int& off) {
         const int t = j * BN + lane_box * a.box;
         if (j < p.s.nt_ctx && j < p.t1 && lane_box * a.box < BN && t < p.s.ctx) {
           blk = table[t / a.bs];
@@ -427,8 +446,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       int next_blk = 0, next_off = 0;
-      if (a.box > 0) locate(p.t0, next_blk, next_off);
-      for (int k = 0; !is_v && k <= int(p.two); ++k, ++qc) {
+      if (a.box > 0) block_of(p.t0, next_blk, next_off);
+      for (int k = 0; !is_v && k <= int(p.two()); ++k, ++qc) {
         const int node0 = (2 * p.pair + k) * a.nodes, nodes = min(p.s.n - node0, a.nodes);
         uint8_t* dq = smem + (qc & 1) * Lay::Q_BYTES;
         if (!wait(&q_empty[qc & 1], ((qc >> 1) & 1) ^ 1)) break;
@@ -455,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int st = g % ST;
         uint8_t* dst = ring + st * Lay::TILE;
         const int blk = next_blk, off = next_off;
-        if (a.box > 0) locate(j + 1, next_blk, next_off);
+        if (a.box > 0) block_of(j + 1, next_blk, next_off);
         if (!wait(&empty[st], ((g / ST) & 1) ^ 1)) break;
         if (j < p.s.nt_ctx) {
           const int t0 = j * BN, valid = min(BN, p.s.ctx - t0);
@@ -527,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t dv0 = smem_desc_sw128(smem_u32(smem + Lay::OFF_V), BN * 128, 1024);
     while (__shfl_sync(0xffffffffu, int(walk.next(a, p)), 0)) {
       const int tiles = __shfl_sync(0xffffffffu, p.t1 - p.t0, 0);
-      const int two = __shfl_sync(0xffffffffu, int(p.two), 0);
+      const int two = __shfl_sync(0xffffffffu, int(p.two()), 0);
       const int k = two ? stream ^ (u0 & 1) : 0;
       const int i0 = two ? 0 : (u0 & 1) ^ stream, di = 2 - two;
       const bool idle = i0 >= tiles;  // a single tile, and the other stream has it
@@ -608,15 +627,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
     const uint32_t tOs = tO + stream * 128 + lane_off;
     const float sl2 = a.scale_log2;
-    bool ok = true;
     int g = 0, u0 = 0, item = 0;  // tiles and units before the piece, pieces
+    // after a wait that ran out (recorded), later ones are skipped
+    bool alive = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-      ok = ok && mbar_wait(bar, parity, a.err);
-      ok = __all_sync(0xffffffffu, ok);
+      if (alive) alive = mbar_wait(bar, parity, a.err);
+      __syncwarp();
     };
-    while (walk.next(a, p)) {
+    bool more = walk.next(a, p);
+    while (more) {
       const int tiles = p.t1 - p.t0;
-      const int k = p.two ? stream ^ (u0 & 1) : 0;  // this stream's row tile
+      const int k = p.two() ? stream ^ (u0 & 1) : 0;  // this stream's row tile
       const int rows = p.rows(a, k);
       const bool live = (warp & 3) * 32 < rows;  // warps without a valid row only keep the barriers going
       const int node = (2 * p.pair + k) * a.nodes + row / a.group;
@@ -624,10 +645,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m_ref = -INFINITY, l0 = 0.f, l1 = 0.f;
       bool odd = false;   // the piece's tree V holds values that are not finite
       bool fresh = true;  // no unit of this stream yet
-      const int i0 = p.two ? 0 : (u0 & 1) ^ stream, di = p.two ? 1 : 2;
+      const int i0 = p.two() ? 0 : (u0 & 1) ^ stream, di = p.two() ? 1 : 2;
       for (int i = i0; i < tiles; i += di) {
-        const int j = p.t0 + i, u = p.two ? u0 + 2 * i + k : u0 + i;
-        const int buf = u & 3, st = (g + i) % ST;
+        const int j = p.t0 + i, u = p.two() ? u0 + 2 * i + k : u0 + i;
+        const int buf = u & 3;
         const uint32_t tS = tmem + buf * BN + lane_off;
         const bool tree = j >= p.s.nt_ctx;
         const int col0 = tree ? (j - p.s.nt_ctx) * BN : j * BN;
@@ -641,11 +662,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           // see them after the last product.  (The stage's phase before this
           // one is complete: S(u) came after P V of unit u - 4, at most four
           // tiles back, whose issuer had waited for every tile before it.)
+          const int st = (g + i) % ST;
           wait(&v_full[st], ((g + i) / ST) & 1);
-          const int tag = p.two ? u0 + 2 * i : u;
-          const int part = p.two ? threadIdx.x : row, parts = p.two ? 256 : 128;
-          if (ok) {
+          const int tag = p.two() ? u0 + 2 * i : u;
+          const int part = p.two() ? threadIdx.x : row, parts = p.two() ? 256 : 128;
+          {
             uint8_t* v = smem + Lay::OFF_V + st * Lay::TILE;
+#pragma unroll 1
             for (int e = part; e < BN * (D / 8); e += parts) {
               const int r = e / (D / 8);
               uint4* w = reinterpret_cast<uint4*>(v + tile_offset(BN, r, e % (D / 8)));
@@ -664,10 +687,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             fence_proxy_async_smem();
           }
           __syncwarp();  // bar.sync and the tcgen05 loads and stores want whole warps
-          bar_sync(p.two ? 3 : 1 + stream, parts);
+          bar_sync(p.two() ? 3 : 1 + stream, parts);
           if (tree) odd = odd || sh.odd[tag & 3] == uint32_t(tag) + 1;
         }
-        if (live && ok) {
+        if (live) {
           uint32_t r[2][32];
           tmem_ld32(tS, r[0]);
           tmem_ld32(tS + 32, r[1]);
@@ -751,14 +774,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         fresh = false;
         tc_fence_before();
         __syncwarp();
-        if (lane == 0 && ok) mbar_arrive(&p_full[buf]);
+        if (lane == 0) mbar_arrive(&p_full[buf]);
       }
-      // the piece's O is complete
-      wait(o_full, item & 1);
+      // find the next piece while the last products run
+      const Piece e = p;
+      more = walk.next(a, p);
+      wait(o_full, item & 1);  // the piece's O is complete
       tc_fence_after();
+      const bool two = e.two(), whole = e.whole();
       float l = l0 + l1, f0 = 1.f, f1 = 0.f, m = m_ref;
-      const bool join = !p.two && tiles > 1;  // both streams hold a part of every row
-      if (!p.two) {
+      const bool join = !two && tiles > 1;  // both streams hold a part of every row
+      if (!two) {
         sh.ml[stream][row] = make_float2(m_ref, l);
         if (row == 0) sh.piece_odd[stream] = odd;
         __syncwarp();
@@ -772,21 +798,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         l = x.y * f0 + y.y * f1;
         odd = sh.piece_odd[0] || sh.piece_odd[1];
       }
-      if (ok && live) {
-        const int64_t rec =
-            ((2 * int64_t(blockIdx.x) + (p.starts ? 1 : 0)) * 2 + k) * a.part_rows + row;
-        const float inv = p.whole ? (l > 0.f || l != l ? 1.0f / l : 0.f) : 1.0f;
-        const int qh = p.h * a.group + row % a.group;
-        uint16_t* orow = reinterpret_cast<uint16_t*>(a.out) + int64_t(p.s.lo + node) * a.out_r + int64_t(qh) * a.out_h;
-        float* prow = a.part_o + rec * D;
+      if (live) {
+        const int slot = (2 * int(blockIdx.x) + (e.starts() ? 1 : 0)) * 2 + k;
+        const float inv = whole ? (l > 0.f || l != l ? 1.0f / l : 0.f) : 1.0f;
+        const int qh = e.h * a.group + row % a.group;
+        uint16_t* orow = reinterpret_cast<uint16_t*>(a.out) + int64_t(e.s.lo + node) * a.out_r + int64_t(qh) * a.out_h;
+        float4* prow = a.part_o + int64_t(slot) * (D / 4) * a.part_rows + row;
         // two row tiles: all columns of the own one; else half of the columns of both streams' O
         constexpr int NC = D / 32;
-        const int c_lo = p.two ? 0 : stream * (NC / 2), c_hi = p.two ? NC : c_lo + NC / 2;
+        const int c_lo = two ? 0 : stream * (NC / 2), c_hi = two ? NC : c_lo + NC / 2;
 #pragma unroll 1
         for (int c = c_lo; c < c_hi; ++c) {
           uint32_t o[32];
           __syncwarp();
-          if (p.two) {
+          if (two) {
             tmem_ld32(tOs + c * 32, o);
             tmem_wait_ld();
           } else {
@@ -797,30 +822,30 @@ __global__ void __launch_bounds__(kThreads, 1)
               tmem_wait_ld();
               const float fa = (u0 & 1) ? f1 : f0, fb = (u0 & 1) ? f0 : f1;
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                o[e] = __float_as_uint(fmaf(__uint_as_float(o[e]), fa, __uint_as_float(o2[e]) * fb));
+              for (int x = 0; x < 32; ++x)
+                o[x] = __float_as_uint(fmaf(__uint_as_float(o[x]), fa, __uint_as_float(o2[x]) * fb));
             } else {
               tmem_wait_ld();
             }
           }
           if (mine && odd) {
-            const int from = max(p.t0 - p.s.nt_ctx, 0) * BN, upto = min((p.t1 - p.s.nt_ctx) * BN, p.s.n);
+            const int from = max(e.t0 - e.s.nt_ctx, 0) * BN, upto = min((e.t1 - e.s.nt_ctx) * BN, e.s.n);
             for (int t = from; t < upto; ++t) {
               const bool sees =
                   a.mask == nullptr
                       ? t <= node
                       : (t >> 5) < a.words &&
-                            (uint32_t(a.mask[int64_t(p.s.lo + node) * a.words + (t >> 5)]) >> (t & 31)) & 1u;
+                            (uint32_t(a.mask[int64_t(e.s.lo + node) * a.words + (t >> 5)]) >> (t & 31)) & 1u;
               if (!sees) continue;
-              const T* v = reinterpret_cast<const T*>(a.vt) + int64_t(p.s.lo + t) * a.vt_r + p.h * a.vt_h + c * 32;
+              const T* v = reinterpret_cast<const T*>(a.vt) + int64_t(e.s.lo + t) * a.vt_r + e.h * a.vt_h + c * 32;
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const float x = as_float<T>(v[e]);
-                if (!(fabsf(x) < INFINITY)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
+              for (int x = 0; x < 32; ++x) {
+                const float y = as_float<T>(v[x]);
+                if (!(fabsf(y) < INFINITY)) o[x] = __float_as_uint(__uint_as_float(o[x]) + y);
               }
             }
           }
-          if (mine && p.whole) {
+          if (mine && whole) {
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
               uint4 w;
@@ -833,18 +858,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else if (mine) {
 #pragma unroll
             for (int v = 0; v < 8; ++v)
-              *reinterpret_cast<uint4*>(prow + c * 32 + v * 4) =
-                  make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+              prow[(c * 8 + v) * a.part_rows] =
+                  make_float4(__uint_as_float(o[4 * v]), __uint_as_float(o[4 * v + 1]), __uint_as_float(o[4 * v + 2]),
+                              __uint_as_float(o[4 * v + 3]));
           }
         }
-        if (mine && !p.whole && (p.two || stream == 0)) a.part_ml[rec] = make_float2(m, l);
+        if (mine && !whole && (two || stream == 0)) a.part_ml[int64_t(slot) * a.part_rows + row] = make_float2(m, l);
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0 && ok) mbar_arrive(o_empty);
+      if (lane == 0) mbar_arrive(o_empty);
       ++item;
       g += tiles;
-      u0 += tiles * (p.two ? 2 : 1);
+      u0 += tiles * (two ? 2 : 1);
     }
   }
   __syncwarp();
@@ -857,103 +883,122 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the records of items that several CTAs shared: one warp per (row,
-// head), records in the order of their tiles.  Padding rows become zero.
+// Joins the records of items that several CTAs shared.  An item has a worker
+// for each CTA whose share begins inside it (an item that no share begins
+// inside of, or only at its first tile and that ends before the next, was
+// whole), so the work is spread like the main kernel's.  A worker joins its
+// part of the item's rows: first all records' maxima and sums, then their O in
+// the order of the tiles.  Rows of no request become zero.
+constexpr int kMergeThreads = 256;
+constexpr int kMergeSplit = 2;     // CTAs a worker
+constexpr int kMergeRecords = 2048;  // (row, record) pairs of one round; more than an item has records (3 a CTA)
+
 template <typename T, int D>
-__global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs a) {
+__global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArgs a) {
+  constexpr int L = D / 4;  // lanes of a row
+  __shared__ float2 s_ml[kMergeRecords];
+  __shared__ float s_inv[2 * BM];
+  __shared__ int s_slot[kMergeRecords];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  {  // inputs only, so before the wait
+    const int lo = min(max(a.indptr[0], 0), a.R), hi = min(max(a.indptr[a.B], lo), a.R);
+    const int hq = a.hkv * a.group, free_rows = lo + a.R - hi;
+    const int64_t step = int64_t(gridDim.x) * kMergeThreads;
+    for (int64_t e = int64_t(blockIdx.x) * kMergeThreads + tid; e < int64_t(free_rows) * hq * (D / 8); e += step) {
+      const int64_t rh = e / (D / 8);
+      int r = int(rh / hq);
+      r = r < lo ? r : hi + r - lo;
+      *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + r * a.out_r + (rh % hq) * a.out_h +
+                                (e % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
+    }
+  }
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t w = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  const int hq = a.hkv * a.group;
-  const int r = int(w / hq), qh = int(w % hq);
-  if (r >= a.R) return;
-  constexpr int E = D / 32;
-  T* out = reinterpret_cast<T*>(a.out) + r * a.out_r + qh * a.out_h + lane * E;
-  auto store = [&](const float (&v)[E]) {
-#pragma unroll
-    for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(out + e) = pack2<T>(v[e], v[e + 1]);
+  const int cta = blockIdx.x / kMergeSplit, part = blockIdx.x % kMergeSplit;
+  const int4 meta = a.meta[cta];
+  if (!meta.w) return;
+  const int share = meta.z, at = cta * share;
+  Piece p;
+  p.s = request_shape(a, meta.x);
+  const Segments seg(p.s, share);
+  locate(p.s, seg, at - meta.y, p);
+  // segment i of the item: its first tile's number, the CTAs [first, last] that hold it
+  const int head = meta.y + p.h * p.s.pairs * p.s.nt;
+  auto first_tile = [&](int i) { return head + seg.start(i) * p.s.pairs + p.pair * seg.length(i); };
+  int workers = 0, rank = 0, records = 0;
+  for (int i = 0; i < seg.count; ++i) {
+    const int x = first_tile(i), y = x + seg.length(i) - 1;
+    if (i == p.segment) rank = workers + cta - (x + share - 1) / share;
+    workers += y / share - (x + share - 1) / share + 1;
+    records += y / share - x / share + 1;
+  }
+  if (records == 1 || records > kMergeRecords) return;  // one CTA had the whole item
+  rank = rank * kMergeSplit + part;
+  workers *= kMergeSplit;
+  const int rows0 = p.rows(a, 0), rows = rows0 + (p.two() ? p.rows(a, 1) : 0);
+  const int row_lo = int(int64_t(rows) * rank / workers), row_hi = int(int64_t(rows) * (rank + 1) / workers);
+  const int batch = max(1, min(kMergeRecords / records, 2 * BM));  // rows of a round
+  // slot of record k: records are numbered along the segments
+  auto slot_of = [&](int k) {
+    int i = 0;
+    if (seg.count > 1)
+      for (;; ++i) {
+        const int x = first_tile(i), n = (x + seg.length(i) - 1) / share - x / share + 1;
+        if (k < n) break;
+        k -= n;
+      }
+    return (2 * (first_tile(i) / share + k) + (k == 0 ? 1 : 0)) * 2;
   };
-  // the last request with indptr[b] <= r
-  int b = 0;
-  for (int hi = a.B; hi - b > 1;) {
-    const int mid = (b + hi) >> 1;
-    if (a.indptr[mid] <= r) b = mid; else hi = mid;
-  }
-  const Shape s = request_shape(a, b);
-  float acc[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  if (r >= s.lo + s.n || r < s.lo) {
-    store(acc);
-    return;
-  }
-  const int64_t share = a.base[a.B];
-  const int h = qh / a.group, node = r - s.lo, mi = node / a.nodes, pair = mi >> 1;
-  const int row = (node % a.nodes) * a.group + qh % a.group;
-  if (share <= 0) return;
-  const Segments seg(s, share);
-  const int64_t first = a.base[b] + int64_t(h) * s.pairs * s.nt;
-  auto segment_first = [&](int i) { return first + int64_t(seg.start(i)) * s.pairs + int64_t(pair) * seg.length(i); };
-  // Records by number: a segment of an item with several is at most twice a
-  // share long, so it touches up to three CTAs, four numbers each; a single
-  // segment has one for each of its CTAs.
-  const int64_t begin = segment_first(0), end = begin + seg.length(0) - 1;
-  const int width = seg.count == 1 ? int(end / share - begin / share) + 1 : 4;
-  if (seg.count == 1 && width == 1) return;  // one CTA had the whole item
-  float m = -INFINITY, l = 0.f;
-  for (int k0 = 0; k0 < seg.count * width; k0 += 32) {
-    // every lane takes one record's maximum and sum
-    const int k = k0 + lane, i = k / width;
-    int64_t rec = -1;
-    float2 ml = make_float2(-INFINITY, 0.f);
-    if (i < seg.count) {
-      const int64_t g0 = segment_first(i), c0 = g0 / share, c = c0 + k % width;
-      if (c <= (g0 + seg.length(i) - 1) / share && c >= 0 && c < a.ctas) {
-        rec = ((2 * c + (c == c0 ? 1 : 0)) * 2 + (mi & 1)) * a.part_rows + row;
-        ml = a.part_ml[rec];
-      }
+  for (int k = tid; k < records; k += kMergeThreads) s_slot[k] = slot_of(k);
+  __syncthreads();
+  for (int r0 = row_lo; r0 < row_hi; r0 += batch) {
+    const int n = min(batch, row_hi - r0);
+    for (int e = tid; e < n * records; e += kMergeThreads) {
+      const int k = e / n, r = r0 + e % n, tile = r >= rows0;
+      s_ml[(e % n) * records + k] = a.part_ml[int64_t(s_slot[k] + tile) * a.part_rows + r - (tile ? rows0 : 0)];
     }
-    float mx = fmaxf(m, ml.x);
+    __syncthreads();
+    // maxima -> weights, a warp a row
+    for (int r = warp; r < n; r += kMergeThreads / 32) {
+      float2* ml = s_ml + r * records;
+      float m = -INFINITY, l = 0.f;
+      for (int k = lane; k < records; k += 32) m = fmaxf(m, ml[k].x);
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-    const float f = m == -INFINITY ? 0.f : ex2(m - mx);
-    const float weight = ml.x == -INFINITY ? 0.f : ex2(ml.x - mx);
-    float ls = ml.y * weight;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, d);
-    l = l * f + ls;
-    m = mx;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] *= f;
-    // the records' rows in order, four loads in flight
-    uint32_t todo = __ballot_sync(0xffffffffu, rec >= 0);
-    while (todo) {
-      float o[4][E], w[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int from = todo ? __ffs(todo) - 1 : 0;
-        const int64_t at = __shfl_sync(0xffffffffu, rec, from);
-        w[x] = __shfl_sync(0xffffffffu, weight, from);
-        if (!todo) w[x] = 0.f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[x][e] = 0.f;
-        if (todo) {
-          const float* po = a.part_o + at * D + lane * E;
-          if constexpr (E == 4) *reinterpret_cast<float4*>(o[x]) = *reinterpret_cast<const float4*>(po);
-          else *reinterpret_cast<float2*>(o[x]) = *reinterpret_cast<const float2*>(po);
-        }
-        todo &= todo - 1;
+      for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+      for (int k = lane; k < records; k += 32) {
+        const float w = ml[k].x == -INFINITY ? 0.f : ex2(ml[k].x - m);
+        l += w * ml[k].y;
+        ml[k].x = w;
       }
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = fmaf(o[x][e], w[x], acc[e]);
+      for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+      if (lane == 0) s_inv[r] = l > 0.f || l != l ? 1.0f / l : 0.f;
     }
+    __syncthreads();
+    for (int e = tid; e < n * L; e += kMergeThreads) {
+      // neighbouring threads take neighbouring rows, as the records lie
+      const int r = e % n, c = e / n, abs = r0 + r, tile = abs >= rows0;
+      const int row = abs - (tile ? rows0 : 0);
+      const float4* po = a.part_o + int64_t(c) * a.part_rows + row;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int k = 0; k < records; ++k) {
+        const float4 o = po[int64_t(s_slot[k] + tile) * (D / 4) * a.part_rows];
+        const float w = s_ml[r * records + k].x;
+        acc.x = fmaf(o.x, w, acc.x);
+        acc.y = fmaf(o.y, w, acc.y);
+        acc.z = fmaf(o.z, w, acc.z);
+        acc.w = fmaf(o.w, w, acc.w);
+      }
+      const float inv = s_inv[r];
+      const int node = (2 * p.pair + tile) * a.nodes + row / a.group, qh = p.h * a.group + row % a.group;
+      uint2 v;
+      v.x = pack2<T>(acc.x * inv, acc.y * inv);
+      v.y = pack2<T>(acc.z * inv, acc.w * inv);
+      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + int64_t(p.s.lo + node) * a.out_r +
+                                int64_t(qh) * a.out_h + c * 4) = v;
+    }
+    __syncthreads();
   }
-  const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] *= inv;
-  store(acc);
 }
 
 // Tensor map of rows of D elements with up to three outer dimensions, outer
@@ -1011,8 +1056,7 @@ void launch(const CUtensorMap* m, const TreeArgs& a, int grid, cudaStream_t st) 
                                       Layout<D>::SMEM));
   tree_attention_kernel<T, D><<<grid, kThreads, Layout<D>::SMEM, st>>>(m[0], m[1], m[2], m[3], m[4], a);
   KVS_CUDA_CHECK(cudaGetLastError());
-  const int64_t warps = int64_t(a.R) * a.hkv * a.group;
-  launch_pdl(tree_merge_kernel<T, D>, dim3(unsigned((warps + 3) / 4)), dim3(128), 0, st, a);
+  launch_pdl(tree_merge_kernel<T, D>, dim3(unsigned(grid * kMergeSplit)), dim3(kMergeThreads), 0, st, a);
 }
 
 }  // namespace
@@ -1117,10 +1161,12 @@ void paged_tree_attention(torch::Tensor q, torch::Tensor k_tree, torch::Tensor v
   a.part_rows = int(std::min<int64_t>(BM, R * a.group));
   a.ctas = grid;
   const int64_t recs = int64_t(4) * grid * a.part_rows;
-  torch::Tensor scratch = torch::empty({recs * (D + 2) + 2 * (B + 1)}, q.options().dtype(at::kFloat));
-  a.part_o = scratch.data_ptr<float>();
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + recs * D);
-  a.base = reinterpret_cast<int64_t*>(a.part_o + recs * (D + 2));
+  // records (O, then maxima and sums) and the CTAs' places in the schedule, 16-byte words
+  const int64_t words = recs * (D / 4) + (recs + 1) / 2 + grid;
+  torch::Tensor scratch = torch::empty({words * 4}, q.options().dtype(at::kFloat));
+  a.part_o = reinterpret_cast<float4*>(scratch.data_ptr<float>());
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + recs * (D / 4));
+  a.meta = reinterpret_cast<int4*>(a.part_o + recs * (D / 4) + (recs + 1) / 2);
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
   if (dt == at::kBFloat16) {
     if (D == 128) launch<bf16, 128>(m, a, grid, st);

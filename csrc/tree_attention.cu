@@ -547,6 +547,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     while (__shfl_sync(0xffffffffu, int(walk.next(a, p)), 0)) {
       const int tiles = __shfl_sync(0xffffffffu, p.t1 - p.t0, 0);
       const int two = __shfl_sync(0xffffffffu, int(p.two()), 0);
+      // tokens from the piece's first tile to the end of the context, the
+      // tiles that hold them, and tree rows from the first tree tile on
+      const int ctx_left = __shfl_sync(0xffffffffu, p.s.ctx - p.t0 * BN, 0);
+      const int nt_ctx = __shfl_sync(0xffffffffu, max(p.s.nt_ctx - p.t0, 0), 0);
+      const int n_left = __shfl_sync(0xffffffffu, p.s.n - max(p.t0 - p.s.nt_ctx, 0) * BN, 0);
       const int k = two ? stream ^ (u0 & 1) : 0;
       const int i0 = two ? 0 : (u0 & 1) ^ stream, di = 2 - two;
       const bool idle = i0 >= tiles;  // a single tile, and the other stream has it
@@ -591,6 +596,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           wait(&v_full[st], (g / ST) & 1);
           if (two || (i & 1) == i0) {
             const int u = two ? u0 + 2 * i + k : u0 + i;
+            // rows past the end take no part, but for the rest of the last 16
+            const int steps = (min(BN, i < nt_ctx ? ctx_left - i * BN : n_left - (i - nt_ctx) * BN) + 15) / 16;
             wait(&p_full[u & 3], (u >> 2) & 1);
             tc_fence_after();
             if (elect_one()) {
@@ -598,7 +605,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               const uint32_t to = tm + 4 * BN + stream * 128, tp = tm + (u & 3) * BN;
 #pragma unroll
               for (int kk = 0; kk < BN / 16; ++kk)
-                umma_f16_ta(to, tp + kk * 8, dv + kk * (2048 >> 4), idesc_pv, (i != i0 || kk > 0) ? 1u : 0u);
+                if (kk < steps)
+                  umma_f16_ta(to, tp + kk * 8, dv + kk * (2048 >> 4), idesc_pv, (i != i0 || kk > 0) ? 1u : 0u);
               umma_commit(&pv_done[u & 3]);
               umma_commit(&v_empty[st]);
               if (i + di >= tiles) umma_commit(o_full);
@@ -643,6 +651,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int node = (2 * p.pair + k) * a.nodes + row / a.group;
       const bool mine = row < rows;
       float m_ref = -INFINITY, l0 = 0.f, l1 = 0.f;
+      // mask words of the piece's first tree tile, read ahead
+      const int tree0 = max(p.t0, p.s.nt_ctx);
+      uint32_t ahead[2] = {0u, 0u};
+      if (tree0 < p.t1 && mine && a.mask != nullptr) {
+        const int word = (tree0 - p.s.nt_ctx) * (BN / 32);
+        const int32_t* mp = a.mask + int64_t(p.s.lo + node) * a.words;
+        if (word < a.words) ahead[0] = uint32_t(mp[word]);
+        if (word + 1 < a.words) ahead[1] = uint32_t(mp[word + 1]);
+      }
       bool odd = false;   // the piece's tree V holds values that are not finite
       bool fresh = true;  // no unit of this stream yet
       const int i0 = p.two() ? 0 : (u0 & 1) ^ stream, di = p.two() ? 1 : 2;
@@ -667,14 +684,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int tag = p.two() ? u0 + 2 * i : u;
           const int part = p.two() ? threadIdx.x : row, parts = p.two() ? 256 : 128;
           {
+            // the products read whole steps of 16 rows: clear the rest of the
+            // last one; look through the rows of a tree tile
             uint8_t* v = smem + Lay::OFF_V + st * Lay::TILE;
-#pragma unroll 1
-            for (int e = part; e < BN * (D / 8); e += parts) {
-              const int r = e / (D / 8);
-              uint4* w = reinterpret_cast<uint4*>(v + tile_offset(BN, r, e % (D / 8)));
-              if (r >= valid) {
+            const int from = tree ? 0 : valid * (D / 8), upto = (valid + 15) / 16 * 16 * (D / 8);
+#pragma unroll 2
+            for (int e = from + part; e < upto; e += parts) {
+              uint4* w = reinterpret_cast<uint4*>(v + tile_offset(BN, e / (D / 8), e % (D / 8)));
+              if (e >= valid * (D / 8)) {
                 *w = make_uint4(0, 0, 0, 0);
-              } else if (tree) {
+              } else {
                 const uint4 x = *w;
                 if (odd2<T>(x.x) || odd2<T>(x.y) || odd2<T>(x.z) || odd2<T>(x.w)) {
                   uint16_t* h = reinterpret_cast<uint16_t*>(w);
@@ -704,7 +723,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (tree) {
                 if (a.mask != nullptr) {
                   const int word = (col0 >> 5) + w;
-                  in &= mine && word < a.words ? uint32_t(a.mask[int64_t(p.s.lo + node) * a.words + word]) : 0u;
+                  if (j == tree0) in &= ahead[w];
+                  else in &= mine && word < a.words ? uint32_t(a.mask[int64_t(p.s.lo + node) * a.words + word]) : 0u;
                 } else {
                   const int upto = node - col0 - 32 * w + 1;  // rows up to itself
                   in &= upto >= 32 ? 0xffffffffu : upto <= 0 ? 0u : (1u << upto) - 1u;
@@ -779,12 +799,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       // find the next piece while the last products run
       const Piece e = p;
       more = walk.next(a, p);
-      wait(o_full, item & 1);  // the piece's O is complete
-      tc_fence_after();
       const bool two = e.two(), whole = e.whole();
       float l = l0 + l1, f0 = 1.f, f1 = 0.f, m = m_ref;
       const bool join = !two && tiles > 1;  // both streams hold a part of every row
       if (!two) {
+        // every warp has read the piece before's (it gave O back after that)
+        wait(o_empty, (item & 1) ^ 1);
         sh.ml[stream][row] = make_float2(m_ref, l);
         if (row == 0) sh.piece_odd[stream] = odd;
         __syncwarp();
@@ -798,6 +818,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         l = x.y * f0 + y.y * f1;
         odd = sh.piece_odd[0] || sh.piece_odd[1];
       }
+      wait(o_full, item & 1);  // the piece's O is complete
+      tc_fence_after();
       if (live) {
         const int slot = (2 * int(blockIdx.x) + (e.starts() ? 1 : 0)) * 2 + k;
         const float inv = whole ? (l > 0.f || l != l ? 1.0f / l : 0.f) : 1.0f;
@@ -827,6 +849,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             } else {
               tmem_wait_ld();
             }
+          }
+          if (c + 1 == c_hi) {  // O is read: the next piece's products may begin
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_empty);
           }
           if (mine && odd) {
             const int from = max(e.t0 - e.s.nt_ctx, 0) * BN, upto = min((e.t1 - e.s.nt_ctx) * BN, e.s.n);
@@ -865,9 +892,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (mine && !whole && (two || stream == 0)) a.part_ml[int64_t(slot) * a.part_rows + row] = make_float2(m, l);
       }
-      tc_fence_before();
+      if (!live && lane == 0) mbar_arrive(o_empty);
       __syncwarp();
-      if (lane == 0) mbar_arrive(o_empty);
       ++item;
       g += tiles;
       u0 += tiles * (two ? 2 : 1);
@@ -886,25 +912,23 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Joins the records of items that several CTAs shared.  An item has a worker
 // for each CTA whose share begins inside it (an item that no share begins
 // inside of, or only at its first tile and that ends before the next, was
-// whole), so the work is spread like the main kernel's.  A worker joins its
-// part of the item's rows: first all records' maxima and sums, then their O in
-// the order of the tiles.  Rows of no request become zero.
+// whole), so the work is spread like the main kernel's.  A warp joins two
+// neighbouring rows at a time, records in the order of their tiles, sixteen in
+// a round: their maxima and sums first (one lane a record and row), then O,
+// with the loads of four records in flight.  Rows of no request become zero.
+// All of it is a few dependent reads from L2: bound by latency.
 constexpr int kMergeThreads = 256;
-constexpr int kMergeSplit = 2;     // CTAs a worker
-constexpr int kMergeRecords = 2048;  // (row, record) pairs of one round; more than an item has records (3 a CTA)
+constexpr int kMergeSplit = 4;  // CTAs a worker
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArgs a) {
-  constexpr int L = D / 4;  // lanes of a row
-  __shared__ float2 s_ml[kMergeRecords];
-  __shared__ float s_inv[2 * BM];
-  __shared__ int s_slot[kMergeRecords];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int NC = D / 64;  // float4 of a row that a lane takes
+  const int lane = threadIdx.x & 31, rr = lane & 1, c0 = lane >> 1;
   {  // inputs only, so before the wait
     const int lo = min(max(a.indptr[0], 0), a.R), hi = min(max(a.indptr[a.B], lo), a.R);
     const int hq = a.hkv * a.group, free_rows = lo + a.R - hi;
     const int64_t step = int64_t(gridDim.x) * kMergeThreads;
-    for (int64_t e = int64_t(blockIdx.x) * kMergeThreads + tid; e < int64_t(free_rows) * hq * (D / 8); e += step) {
+    for (int64_t e = int64_t(blockIdx.x) * kMergeThreads + threadIdx.x; e < int64_t(free_rows) * hq * (D / 8); e += step) {
       const int64_t rh = e / (D / 8);
       int r = int(rh / hq);
       r = r < lo ? r : hi + r - lo;
@@ -921,83 +945,101 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArg
   p.s = request_shape(a, meta.x);
   const Segments seg(p.s, share);
   locate(p.s, seg, at - meta.y, p);
-  // segment i of the item: its first tile's number, the CTAs [first, last] that hold it
   const int head = meta.y + p.h * p.s.pairs * p.s.nt;
   auto first_tile = [&](int i) { return head + seg.start(i) * p.s.pairs + p.pair * seg.length(i); };
   int workers = 0, rank = 0, records = 0;
+#pragma unroll 1
   for (int i = 0; i < seg.count; ++i) {
     const int x = first_tile(i), y = x + seg.length(i) - 1;
-    if (i == p.segment) rank = workers + cta - (x + share - 1) / share;
-    workers += y / share - (x + share - 1) / share + 1;
-    records += y / share - x / share + 1;
+    const int first = x / share, last = y / share, begins = first + (first * share < x ? 1 : 0);
+    if (i == p.segment) rank = workers + cta - begins;
+    workers += last - begins + 1;
+    records += last - first + 1;
   }
-  if (records == 1 || records > kMergeRecords) return;  // one CTA had the whole item
-  rank = rank * kMergeSplit + part;
-  workers *= kMergeSplit;
+  if (records == 1) return;  // one CTA had the whole item
   const int rows0 = p.rows(a, 0), rows = rows0 + (p.two() ? p.rows(a, 1) : 0);
-  const int row_lo = int(int64_t(rows) * rank / workers), row_hi = int(int64_t(rows) * (rank + 1) / workers);
-  const int batch = max(1, min(kMergeRecords / records, 2 * BM));  // rows of a round
-  // slot of record k: records are numbered along the segments
-  auto slot_of = [&](int k) {
-    int i = 0;
-    if (seg.count > 1)
-      for (;; ++i) {
-        const int x = first_tile(i), n = (x + seg.length(i) - 1) / share - x / share + 1;
-        if (k < n) break;
-        k -= n;
-      }
-    return (2 * (first_tile(i) / share + k) + (k == 0 ? 1 : 0)) * 2;
-  };
-  for (int k = tid; k < records; k += kMergeThreads) s_slot[k] = slot_of(k);
-  __syncthreads();
-  for (int r0 = row_lo; r0 < row_hi; r0 += batch) {
-    const int n = min(batch, row_hi - r0);
-    for (int e = tid; e < n * records; e += kMergeThreads) {
-      const int k = e / n, r = r0 + e % n, tile = r >= rows0;
-      s_ml[(e % n) * records + k] = a.part_ml[int64_t(s_slot[k] + tile) * a.part_rows + r - (tile ? rows0 : 0)];
-    }
-    __syncthreads();
-    // maxima -> weights, a warp a row
-    for (int r = warp; r < n; r += kMergeThreads / 32) {
-      float2* ml = s_ml + r * records;
-      float m = -INFINITY, l = 0.f;
-      for (int k = lane; k < records; k += 32) m = fmaxf(m, ml[k].x);
+  const int stride = workers * kMergeSplit * (kMergeThreads / 32);
+#pragma unroll 1
+  for (int pr = (rank * kMergeSplit + part) * (kMergeThreads / 32) + (threadIdx.x >> 5); 2 * pr < rows; pr += stride) {
+    const int abs = min(2 * pr + rr, rows - 1), tile = abs >= rows0, row = abs - (tile ? rows0 : 0);
+    float m = -INFINITY, l = 0.f;
+    float4 acc[NC];
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-      for (int k = lane; k < records; k += 32) {
-        const float w = ml[k].x == -INFINITY ? 0.f : ex2(ml[k].x - m);
-        l += w * ml[k].y;
-        ml[k].x = w;
+    for (int i = 0; i < NC; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int k0 = 0; k0 < records; k0 += 16) {
+      int k = k0 + c0, slot = -1;
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (k < records) {
+        // records are numbered along the segments
+        int first = first_tile(0) / share;
+        if (seg.count > 1) {
+#pragma unroll 1
+          for (int i = 0;; ++i) {
+            const int x = first_tile(i);
+            first = x / share;
+            const int n = (x + seg.length(i) - 1) / share - first + 1;
+            if (k < n || i + 1 == seg.count) break;
+            k -= n;
+          }
+        }
+        slot = (2 * (first + k) + (k == 0 ? 1 : 0)) * 2 + tile;
+        ml = a.part_ml[int64_t(slot) * a.part_rows + row];
       }
+      float mx = fmaxf(m, ml.x);
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-      if (lane == 0) s_inv[r] = l > 0.f || l != l ? 1.0f / l : 0.f;
-    }
-    __syncthreads();
-    for (int e = tid; e < n * L; e += kMergeThreads) {
-      // neighbouring threads take neighbouring rows, as the records lie
-      const int r = e % n, c = e / n, abs = r0 + r, tile = abs >= rows0;
-      const int row = abs - (tile ? rows0 : 0);
-      const float4* po = a.part_o + int64_t(c) * a.part_rows + row;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int k = 0; k < records; ++k) {
-        const float4 o = po[int64_t(s_slot[k] + tile) * (D / 4) * a.part_rows];
-        const float w = s_ml[r * records + k].x;
-        acc.x = fmaf(o.x, w, acc.x);
-        acc.y = fmaf(o.y, w, acc.y);
-        acc.z = fmaf(o.z, w, acc.z);
-        acc.w = fmaf(o.w, w, acc.w);
+      for (int d = 16; d > 1; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+      const float f = m == -INFINITY ? 0.f : ex2(m - mx), w = ml.x == -INFINITY ? 0.f : ex2(ml.x - mx);
+      float sum = ml.y * w;
+#pragma unroll
+      for (int d = 16; d > 1; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      l = l * f + sum;
+      m = mx;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        acc[i].x *= f;
+        acc[i].y *= f;
+        acc[i].z *= f;
+        acc[i].w *= f;
       }
-      const float inv = s_inv[r];
+      const int n = min(16, records - k0);
+#pragma unroll 1
+      for (int x = 0; x < n; x += 4) {
+        float4 o[4][NC];
+        float wx[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          wx[y] = __shfl_sync(0xffffffffu, w, (2 * (x + y) + rr) & 31);
+          const int s = __shfl_sync(0xffffffffu, slot, (2 * (x + y) + rr) & 31);
+#pragma unroll
+          for (int i = 0; i < NC; ++i)
+            o[y][i] = x + y < n ? a.part_o[(int64_t(s) * (D / 4) + c0 + 16 * i) * a.part_rows + row]
+                                : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+#pragma unroll
+          for (int i = 0; i < NC; ++i) {
+            acc[i].x = fmaf(o[y][i].x, wx[y], acc[i].x);
+            acc[i].y = fmaf(o[y][i].y, wx[y], acc[i].y);
+            acc[i].z = fmaf(o[y][i].z, wx[y], acc[i].z);
+            acc[i].w = fmaf(o[y][i].w, wx[y], acc[i].w);
+          }
+      }
+    }
+    if (2 * pr + rr < rows) {
+      const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
       const int node = (2 * p.pair + tile) * a.nodes + row / a.group, qh = p.h * a.group + row % a.group;
-      uint2 v;
-      v.x = pack2<T>(acc.x * inv, acc.y * inv);
-      v.y = pack2<T>(acc.z * inv, acc.w * inv);
-      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + int64_t(p.s.lo + node) * a.out_r +
-                                int64_t(qh) * a.out_h + c * 4) = v;
+      uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + int64_t(p.s.lo + node) * a.out_r + int64_t(qh) * a.out_h;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        uint2 v;
+        v.x = pack2<T>(acc[i].x * inv, acc[i].y * inv);
+        v.y = pack2<T>(acc[i].z * inv, acc[i].w * inv);
+        *reinterpret_cast<uint2*>(out + (c0 + 16 * i) * 4) = v;
+      }
     }
-    __syncthreads();
+    __syncwarp();
   }
 }
 

@@ -7,6 +7,15 @@
 //   x = x + bias(v);   grammar bit of v clear:  x = -inf
 // seen / count run over the request's committed tokens (count only from the
 // end of its prompt) and over the drafted tokens on the row's own tree path.
+//
+// Every logit is read and written once: bound by HBM for many rows, by
+// latency for one.  A CTA takes a slice of the vocabulary for a few rows: it
+// counts the request's tokens that fall into the slice in shared memory (a
+// word an entry, integer atomics, so the order does not matter), once for all
+// rows of a request, and marks the entries that any rule touches in a bit
+// map.  The rows then stream through 16-byte loads and stores; eight entries
+// whose bits are clear cost two bit tests, the others take the slow path.
+// A row's path tokens are added before it and taken back after it.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -17,9 +26,15 @@
 namespace kvs {
 namespace {
 
-constexpr int kRuleThreads = 256;
-constexpr int kChunk = 4096;
+constexpr int kRuleThreads = 512;
+constexpr int kMaxSlice = 16384;  // entries: 64 KB of counts, two CTAs on an SM
+constexpr int kMinSlice = 1024;
+constexpr int kMaxBias = 2047;
+// a count word: bit 31 seen in the prompt, bits 20..30 bias number + 1, then
+// the count of generated occurrences
 constexpr uint32_t kSeen = 0x80000000u;
+constexpr int kBiasShift = 20;
+constexpr uint32_t kCountMask = (1u << kBiasShift) - 1u;
 
 struct RuleArgs {
   const void* logits;
@@ -43,7 +58,8 @@ struct RuleArgs {
   const int32_t* allowed_index;
   const int32_t *drafts, *indptr, *mask, *positions;
   int mask_words;
-  unsigned long long* best;
+  int slice, slices, rows_per_cta;
+  unsigned long long* best;  // [R, slices]
 };
 
 template <typename T>
@@ -70,97 +86,215 @@ __device__ __forceinline__ unsigned long long greedy_key(float x, int v) {
   return (uint64_t(o) << 32) | uint32_t(~v);
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kRuleThreads) logits_rules_kernel(RuleArgs a) {
-  __shared__ uint32_t s_count[kChunk];
-  __shared__ float s_bias[kChunk];
+__global__ void __launch_bounds__(kRuleThreads, 2) logits_rules_kernel(const RuleArgs a) {
+  pdl_trigger();
+  constexpr int VEC = 16 / sizeof(T);
+  extern __shared__ uint32_t sm[];
   __shared__ unsigned long long s_best[kRuleThreads / 32];
-  const int r = blockIdx.y, v0 = blockIdx.x * kChunk, nv = min(kChunk, a.V - v0);
-  const int id0 = a.vocab_begin + v0;
-  const int b = a.request ? a.request[r] : r;
-  const bool has = b >= 0 && b < a.B;
-  for (int i = threadIdx.x; i < kChunk; i += kRuleThreads) {
-    s_count[i] = 0;
-    s_bias[i] = 0.f;
-  }
-  __syncthreads();
-  const int prompt = has && a.prompt ? a.prompt[b] : 0;
-  if (has && a.tokens) {
-    const int len = min(a.lens[b], a.tokens_len);
-    for (int i = threadIdx.x; i < len; i += kRuleThreads) {
-      const int v = a.tokens[b * a.tokens_stride + i] - id0;
-      if (v >= 0 && v < nv) {
-        atomicOr(&s_count[v], kSeen);
-        if (i >= prompt) atomicAdd(&s_count[v], 1u);
+  uint32_t* s_count = sm;                     // [slice]
+  uint32_t* s_bits = s_count + a.slice;       // [slice / 32 + 1] entries that a rule may change
+  float* s_bias = reinterpret_cast<float*>(s_bits + a.slice / 32 + 1);  // [num_bias]
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int v0 = blockIdx.x * a.slice, nv = min(a.slice, a.V - v0), id0 = a.vocab_begin + v0;
+  const int row0 = blockIdx.y * a.rows_per_cta, row1 = min(row0 + a.rows_per_cta, a.R);
+  int counted = -1;  // request whose tokens the table holds
+  for (int r = row0; r < row1; ++r) {
+    const int b = a.request ? a.request[r] : r;
+    const bool has = b >= 0 && b < a.B;
+    const int prompt = has && a.prompt ? a.prompt[b] : 0;
+    if (has && b != counted) {
+      for (int i = tid; i < a.slice / 4; i += kRuleThreads) reinterpret_cast<uint4*>(s_count)[i] = make_uint4(0, 0, 0, 0);
+      for (int i = tid; i <= a.slice / 32; i += kRuleThreads) s_bits[i] = 0;
+      __syncthreads();
+      if (a.tokens) {
+        const int len = min(a.lens[b], a.tokens_len);
+        const int32_t* tok = a.tokens + b * a.tokens_stride;
+#pragma unroll 8
+        for (int i = tid; i < len; i += kRuleThreads) {
+          const uint32_t v = uint32_t(tok[i]) - uint32_t(id0);
+          if (v < uint32_t(nv)) {
+            if (i >= prompt) atomicAdd(&s_count[v], 1u);
+            else atomicOr(&s_count[v], kSeen);
+            atomicOr(&s_bits[v >> 5], 1u << (v & 31));
+          }
+        }
       }
-    }
-  }
-  if (has && a.drafts) {
-    const int lo = min(max(a.indptr[b], 0), a.R), n = min(a.indptr[b + 1], a.R) - lo;
-    for (int j = threadIdx.x; j < n; j += kRuleThreads) {
-      const bool on = a.mask ? j < 32 * a.mask_words && (a.mask[int64_t(r) * a.mask_words + (j >> 5)] >> (j & 31)) & 1
-                             : lo + j <= r;
-      const int v = a.drafts[lo + j] - id0;
-      if (on && v >= 0 && v < nv) {
-        atomicOr(&s_count[v], kSeen);
-        if (a.positions[lo + j] >= prompt) atomicAdd(&s_count[v], 1u);
+      if (a.num_bias && tid < 32) {
+        // in the order of the list, so that an id listed several times gets
+        // the same sum every time; the first of equal ids owns the sum
+        for (int i0 = 0; i0 < a.num_bias; i0 += 32) {
+          const int i = i0 + lane;
+          const int id = i < a.num_bias ? a.bias_ids[b * a.bias_stride + i] : -1;
+          const uint32_t v = uint32_t(id) - uint32_t(id0);
+          const bool in = id >= 0 && v < uint32_t(nv);
+          const float value = in ? a.bias_values[b * a.bias_value_stride + i] : 0.f;
+          const uint32_t same = __match_any_sync(0xffffffffu, in ? int(v) : -1 - lane);
+          float sum = 0.f;
+          int number = -1;
+          if (in) {
+            number = int((s_count[v] & ~kSeen) >> kBiasShift) - 1;
+            if (number >= 0) sum = s_bias[number];
+          }
+          for (uint32_t rest = 0xffffffffu; rest; rest &= rest - 1) {
+            const int from = __ffs(rest) - 1;
+            const float x = __shfl_sync(0xffffffffu, value, from);
+            if ((same >> from) & 1u) sum = __fadd_rn(sum, x);
+          }
+          if (in && __ffs(same) - 1 == lane) {
+            if (number < 0) {
+              number = i;
+              atomicOr(&s_count[v], uint32_t(i + 1) << kBiasShift);
+              atomicOr(&s_bits[v >> 5], 1u << (v & 31));
+            }
+            s_bias[number] = sum;
+          }
+          __syncwarp();
+        }
       }
+      counted = b;
     }
-  }
-  if (has && a.num_bias && threadIdx.x == 0) {
-    for (int i = 0; i < a.num_bias; ++i) {
-      const int id = a.bias_ids[b * a.bias_stride + i], v = id - id0;
-      if (id >= 0 && v >= 0 && v < nv) s_bias[v] += a.bias_values[b * a.bias_value_stride + i];
+    // the row's own path
+    int lo = 0, n = 0;
+    if (has && a.drafts) {
+      lo = min(max(a.indptr[b], 0), a.R);
+      n = min(a.indptr[b + 1], a.R) - lo;
     }
-  }
-  __syncthreads();
-  const float rep = has && a.repetition ? a.repetition[b] : 1.f;
-  const float freq = has && a.frequency ? a.frequency[b] : 0.f;
-  const float pres = has && a.presence ? a.presence[b] : 0.f;
-  int g = -1;
-  if (a.allowed) g = a.allowed_index ? a.allowed_index[r] : r;
-  const int32_t* bits = g >= 0 && g < a.allowed_rows ? a.allowed + g * a.allowed_stride : nullptr;
-  const T* in = reinterpret_cast<const T*>(a.logits) + r * a.in_stride + v0;
-  T* out = reinterpret_cast<T*>(a.out) + r * a.out_stride + v0;
-  unsigned long long best = 0;
-  for (int i = threadIdx.x; i < nv; i += kRuleThreads) {
-    float x = load(in + i);
-    const uint32_t c = s_count[i];
-    if (c & kSeen) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-    const uint32_t count = c & ~kSeen;
-    if (count) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, float(count))), pres);
-    x = __fadd_rn(x, s_bias[i]);
-    if (bits && !((bits[(v0 + i) >> 5] >> ((v0 + i) & 31)) & 1)) x = -INFINITY;
-    const T y = round_to<T>(x);
-    out[i] = y;
-    const unsigned long long key = greedy_key(load(&y), v0 + i);
-    best = key > best ? key : best;
-  }
-  if (a.best) {
+    auto path = [&](auto&& use) {
+      for (int j = tid; j < n; j += kRuleThreads) {
+        const bool on = a.mask ? j < 32 * a.mask_words && (a.mask[int64_t(r) * a.mask_words + (j >> 5)] >> (j & 31)) & 1
+                               : lo + j <= r;
+        const uint32_t v = on ? uint32_t(a.drafts[lo + j]) - uint32_t(id0) : 0xffffffffu;
+        if (v < uint32_t(nv)) use(v, a.positions[lo + j] >= prompt);
+      }
+    };
+    bool lasting = false;
+    path([&](uint32_t v, bool made) {
+      if (made) atomicAdd(&s_count[v], 1u);
+      else lasting = true, atomicOr(&s_count[v], kSeen);
+      atomicOr(&s_bits[v >> 5], 1u << (v & 31));
+    });
+    if (__syncthreads_or(lasting)) counted = -1;  // a prompt token of the path stays in the table
+
+    const float rep = has && a.repetition ? a.repetition[b] : 1.f;
+    const float freq = has && a.frequency ? a.frequency[b] : 0.f;
+    const float pres = has && a.presence ? a.presence[b] : 0.f;
+    int g = -1;
+    if (a.allowed) g = a.allowed_index ? a.allowed_index[r] : r;
+    // grammar words of the slice (slices begin at whole words)
+    const uint32_t* bits =
+        g >= 0 && g < a.allowed_rows ? reinterpret_cast<const uint32_t*>(a.allowed + g * a.allowed_stride) + (v0 >> 5) : nullptr;
+    const T* in = reinterpret_cast<const T*>(a.logits) + r * a.in_stride + v0;
+    T* out = reinterpret_cast<T*>(a.out) + r * a.out_stride + v0;
+    auto rules = [&](float x, int i) {  // entry i of the slice, not masked
+      const uint32_t c = s_count[i], count = c & kCountMask, number = (c & ~kSeen) >> kBiasShift;
+      if ((c & kSeen) || count) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
+      if (count) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, float(count))), pres);
+      if (number) x = __fadd_rn(x, s_bias[number - 1]);
+      return x;
+    };
+    float top = NAN;              // largest value of the 16-byte pieces so far (NaN: none yet, or it is one)
+    unsigned long long best = 0;  // largest key so far
+    auto one = [&](int i) {
+      float x = load(in + i);
+      if (has && (s_bits[i >> 5] >> (i & 31)) & 1u) x = rules(x, i);
+      if (bits && !((bits[i >> 5] >> (i & 31)) & 1u)) x = -INFINITY;
+      const T y = round_to<T>(x);
+      out[i] = y;
+      const unsigned long long key = greedy_key(load(&y), v0 + i);
+      best = key > best ? key : best;
+    };
+    // 16-byte pieces where input and output have one misalignment
+    const int skew = int((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T));
+    const bool wide = (reinterpret_cast<uintptr_t>(in) & 15) == (reinterpret_cast<uintptr_t>(out) & 15);
+    const int head = wide ? min(nv, (VEC - skew) % VEC) : nv, pieces = (nv - head) / VEC;
+    for (int i = tid; i < head; i += kRuleThreads) one(i);
+    for (int i = head + pieces * VEC + tid; i < nv; i += kRuleThreads) one(i);
+#pragma unroll 2
+    for (int p = tid; p < pieces; p += kRuleThreads) {
+      const int i = head + p * VEC, w = i >> 5;
+      uint4 raw = *reinterpret_cast<const uint4*>(in + i);
+      uint32_t touched = 0, free = ~0u;
+      if (has) touched = __funnelshift_r(s_bits[w], s_bits[w + 1], i & 31);
+      if (bits) free = __funnelshift_r(bits[w], (i & 31) + VEC > 32 ? bits[w + 1] : 0u, i & 31);
+      constexpr uint32_t kAll = (1u << VEC) - 1u;
+      T* e = reinterpret_cast<T*>(&raw);
+      if ((touched | ~free) & kAll) {
 #pragma unroll
-    for (int m = 16; m > 0; m >>= 1) {
-      const unsigned long long o = __shfl_xor_sync(0xffffffffu, best, m);
-      best = o > best ? o : best;
+        for (int x = 0; x < VEC; ++x) {
+          if (!((free >> x) & 1u)) e[x] = round_to<T>(-INFINITY);
+          else if ((touched >> x) & 1u) e[x] = round_to<T>(rules(load(e + x), i + x));
+        }
+      }
+      *reinterpret_cast<uint4*>(out + i) = raw;
+      if (a.best) {
+        float mx = load(e);
+#pragma unroll
+        for (int x = 1; x < VEC; ++x) mx = max_nan(mx, load(e + x));
+        if (!(mx <= top)) {  // larger than all before, or NaN, or the first
+          top = mx;
+#pragma unroll
+          for (int x = 0; x < VEC; ++x) {
+            const unsigned long long key = greedy_key(load(e + x), v0 + i + x);
+            best = key > best ? key : best;
+          }
+        }
+      }
     }
-    if ((threadIdx.x & 31) == 0) s_best[threadIdx.x >> 5] = best;
+    if (a.best) {
+#pragma unroll
+      for (int m = 16; m > 0; m >>= 1) {
+        const unsigned long long o = __shfl_xor_sync(0xffffffffu, best, m);
+        best = o > best ? o : best;
+      }
+      if (lane == 0) s_best[tid >> 5] = best;
+    }
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (a.best && tid == 0) {
       for (int w = 1; w < kRuleThreads / 32; ++w) best = s_best[w] > best ? s_best[w] : best;
-      atomicMax(a.best + r, best);
+      a.best[int64_t(r) * a.slices + blockIdx.x] = best;
     }
+    if (counted >= 0 && r + 1 < row1)
+      path([&](uint32_t v, bool) { atomicSub(&s_count[v], 1u); });
+    __syncthreads();
   }
 }
 
-__global__ void greedy_finish_kernel(const unsigned long long* best, int R, int vocab_begin, int32_t* greedy,
-                                     float* value) {
-  const int r = blockIdx.x * blockDim.x + threadIdx.x;
+// Largest key of a row's slices, a warp a row.
+__global__ void __launch_bounds__(128) greedy_finish_kernel(const unsigned long long* best, int R, int slices,
+                                                            int vocab_begin, int32_t* greedy, float* value) {
+  pdl_wait();
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (r >= R) return;
-  const unsigned long long k = best[r];
+  unsigned long long k = 0;
+  for (int i = lane; i < slices; i += 32) {
+    const unsigned long long o = best[int64_t(r) * slices + i];
+    k = o > k ? o : k;
+  }
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) {
+    const unsigned long long o = __shfl_xor_sync(0xffffffffu, k, m);
+    k = o > k ? o : k;
+  }
+  if (lane != 0) return;
   greedy[r] = vocab_begin + int(~uint32_t(k));
   if (value) {
     const uint32_t o = uint32_t(k >> 32);
     value[r] = o == 0xffffffffu ? NAN : ordered_to_float(o);
   }
+}
+
+template <typename T>
+void launch_rules(const RuleArgs& a, dim3 grid, size_t smem, cudaStream_t st) {
+  KVS_CUDA_CHECK(cudaFuncSetAttribute(logits_rules_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+  logits_rules_kernel<T><<<grid, kRuleThreads, smem, st>>>(a);
+  KVS_CUDA_CHECK(cudaGetLastError());
 }
 
 }  // namespace
@@ -223,8 +357,8 @@ void process_logits(torch::Tensor logits, torch::Tensor out, c10::optional<torch
   if (tokens.has_value()) {
     on(*tokens, at::kInt, "process_logits: tokens int32 [B, M]");
     KVS_CHECK_ARG(tokens->dim() == 2 && tokens->size(0) == B && tokens->stride(1) == 1 &&
-                      tokens->size(1) <= INT32_MAX,
-                  "process_logits: tokens int32 [B, M] with contiguous rows");
+                      tokens->size(1) + R < int64_t(kCountMask),
+                  "process_logits: tokens int32 [B, M] with contiguous rows, M below 2^20");
     a.tokens = tokens->data_ptr<int32_t>();
     a.tokens_stride = tokens->stride(0);
     a.tokens_len = int(tokens->size(1));
@@ -236,7 +370,7 @@ void process_logits(torch::Tensor logits, torch::Tensor out, c10::optional<torch
     KVS_CHECK_ARG(bias_ids->dim() == 2 && bias_ids->size(0) == B && bias_values->sizes() == bias_ids->sizes() &&
                       bias_ids->stride(1) == 1 && bias_values->stride(1) == 1,
                   "process_logits: bias_ids and bias_values [B, K] with contiguous rows");
-    KVS_CHECK_ARG(bias_ids->size(1) <= INT32_MAX, "process_logits: too many biases");
+    KVS_CHECK_ARG(bias_ids->size(1) <= kMaxBias, "process_logits: at most 2047 biases a request");
     a.bias_ids = bias_ids->data_ptr<int32_t>();
     a.bias_values = bias_values->data_ptr<float>();
     a.bias_stride = bias_ids->stride(0);
@@ -281,23 +415,30 @@ void process_logits(torch::Tensor logits, torch::Tensor out, c10::optional<torch
   a.drafts = ip(draft_ids);
   a.indptr = ip(indptr);
   a.positions = ip(positions);
+  // Rows of a CTA share one count of their request's tokens, and a wide slice
+  // reads the tokens less often (16384 entries: 8 to 10 times a row); but
+  // first the GPU's 2 x 148 places have to be filled.
+  int64_t slice = kMaxSlice, rows = 8;
+  auto ctas = [&] { return ((V + slice - 1) / slice) * ((R + rows - 1) / rows); };
+  while (rows > 1 && ctas() < 2 * 2 * kNumSMs) rows /= 2;
+  while (slice > kMinSlice && ctas() < 2 * kNumSMs) slice /= 2;
+  a.slice = int(slice);
+  a.slices = int((V + slice - 1) / slice);
+  a.rows_per_cta = int(rows);
+  const dim3 grid{unsigned(a.slices), unsigned((R + rows - 1) / rows)};
+  const size_t smem = size_t(slice + slice / 32 + 1 + a.num_bias) * 4;
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
   torch::Tensor best;
   if (greedy.has_value()) {
-    best = torch::zeros({R}, logits.options().dtype(at::kLong));
+    best = torch::empty({R * a.slices}, logits.options().dtype(at::kLong));
     a.best = reinterpret_cast<unsigned long long*>(best.data_ptr<int64_t>());
   }
-  const dim3 grid(unsigned((V + kChunk - 1) / kChunk), unsigned(R));
-  if (dt == at::kBFloat16)
-    logits_rules_kernel<bf16><<<grid, kRuleThreads, 0, st>>>(a);
-  else if (dt == at::kHalf)
-    logits_rules_kernel<__half><<<grid, kRuleThreads, 0, st>>>(a);
-  else
-    logits_rules_kernel<float><<<grid, kRuleThreads, 0, st>>>(a);
+  if (dt == at::kBFloat16) launch_rules<bf16>(a, grid, smem, st);
+  else if (dt == at::kHalf) launch_rules<__half>(a, grid, smem, st);
+  else launch_rules<float>(a, grid, smem, st);
   if (greedy.has_value())
-    greedy_finish_kernel<<<unsigned((R + 255) / 256), 256, 0, st>>>(a.best, int(R), int(vocab_begin),
-                                                                    greedy->data_ptr<int32_t>(), fp(greedy_val));
-  KVS_CUDA_CHECK(cudaGetLastError());
+    launch_pdl(greedy_finish_kernel, dim3(unsigned((R + 3) / 4)), dim3(128), 0, st, a.best, int(R), a.slices,
+               int(vocab_begin), greedy->data_ptr<int32_t>(), fp(greedy_val));
 }
 
 }  // namespace kvs

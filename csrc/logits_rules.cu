@@ -12,10 +12,12 @@
 // latency for one.  A CTA takes a slice of the vocabulary for a few rows: it
 // counts the request's tokens that fall into the slice in shared memory (a
 // word an entry, integer atomics, so the order does not matter), once for all
-// rows of a request, and marks the entries that any rule touches in a bit
-// map.  The rows then stream through 16-byte loads and stores; eight entries
-// whose bits are clear cost two bit tests, the others take the slow path.
-// A row's path tokens are added before it and taken back after it.
+// rows of a request, and lists the entries that any rule touches.  A row then
+// streams through 16-byte loads and stores with the grammar bits alone, and
+// the listed entries are computed in a second, short pass: with the rules in
+// the stream, a warp took their branches for nearly every piece (512 rows of
+// fp32: 255 us).  A row's path tokens are added before it and taken back
+// after it.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -27,7 +29,7 @@ namespace kvs {
 namespace {
 
 constexpr int kRuleThreads = 512;
-constexpr int kMaxSlice = 16384;  // entries: 64 KB of counts, two CTAs on an SM
+constexpr int kMaxSlice = 16384;  // entries: 64 KB of counts and 32 KB of list, two CTAs on an SM
 constexpr int kMinSlice = 1024;
 constexpr int kMaxBias = 2047;
 // a count word: bit 31 seen in the prompt, bits 20..30 bias number + 1, then
@@ -91,6 +93,63 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either i
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
   return m;
 }
+__device__ __forceinline__ uint32_t order_of(float x) { return isnan(x) ? 0xffffffffu : float_to_ordered(x + 0.0f); }
+
+// 16 bytes of logits: entries whose bit in `keep` is clear become -inf; the
+// largest entry (NaN if there is one).  16-bit types go by pairs.
+template <typename T>
+struct Pack;
+template <>
+struct Pack<float> {
+  static __device__ __forceinline__ uint4 keep(uint4 w, uint32_t k) {
+    w.x = k & 1u ? w.x : 0xff800000u;
+    w.y = k & 2u ? w.y : 0xff800000u;
+    w.z = k & 4u ? w.z : 0xff800000u;
+    w.w = k & 8u ? w.w : 0xff800000u;
+    return w;
+  }
+  static __device__ __forceinline__ float largest(const uint4& w) {
+    return max_nan(max_nan(__uint_as_float(w.x), __uint_as_float(w.y)),
+                   max_nan(__uint_as_float(w.z), __uint_as_float(w.w)));
+  }
+};
+template <uint32_t kNegInf2>
+__device__ __forceinline__ uint4 keep_halves(uint4 w, uint32_t k) {
+  auto pair = [](uint32_t x, uint32_t b) {  // b: two bits
+    const uint32_t m = (b & 1u) * 0xffffu + (b >> 1 & 1u) * 0xffff0000u;
+    return (x & m) | (kNegInf2 & ~m);
+  };
+  return make_uint4(pair(w.x, k), pair(w.y, k >> 2), pair(w.z, k >> 4), pair(w.w, k >> 6));
+}
+template <>
+struct Pack<bf16> {
+  static __device__ __forceinline__ uint4 keep(const uint4& w, uint32_t k) { return keep_halves<0xff80ff80u>(w, k); }
+  static __device__ __forceinline__ float largest(const uint4& w) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
+    const float2 m = __bfloat1622float2(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
+    return max_nan(m.x, m.y);
+  }
+};
+template <>
+struct Pack<__half> {
+  static __device__ __forceinline__ uint4 keep(const uint4& w, uint32_t k) { return keep_halves<0xfc00fc00u>(w, k); }
+  static __device__ __forceinline__ float largest(const uint4& w) {
+    const __half2* h = reinterpret_cast<const __half2*>(&w);
+    const float2 m = __half22float2(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
+    return max_nan(m.x, m.y);
+  }
+};
+
+// Largest of the warp's 64-bit keys.
+__device__ __forceinline__ unsigned long long warp_max(unsigned long long k) {
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, uint32_t(k >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, uint32_t(k >> 32) == hi ? uint32_t(k) : 0u);
+  return (uint64_t(hi) << 32) | lo;
+}
+
+constexpr int kMaxRows = 8;   // rows of a CTA
+constexpr int kBatch = 4;  // 16-byte pieces of a thread in flight
+constexpr int kAhead = 8;  // tokens of a thread read while the table is cleared
 
 template <typename T>
 __global__ void __launch_bounds__(kRuleThreads, 2) logits_rules_kernel(const RuleArgs a) {
@@ -99,42 +158,142 @@ __global__ void __launch_bounds__(kRuleThreads, 2) logits_rules_kernel(const Rul
   extern __shared__ uint32_t sm[];
   __shared__ unsigned long long s_best[kRuleThreads / 32];
   uint32_t* s_count = sm;                     // [slice]
-  uint32_t* s_bits = s_count + a.slice;       // [slice / 32 + 1] entries that a rule may change
-  float* s_bias = reinterpret_cast<float*>(s_bits + a.slice / 32 + 1);  // [num_bias]
+  uint32_t* s_bits = s_count + a.slice;       // [slice / 32 + 4] entries that a rule may change ...
+  uint16_t* s_list = reinterpret_cast<uint16_t*>(s_bits + a.slice / 32 + 4);  // [slice] ... and their list
+  float* s_bias = reinterpret_cast<float*>(s_list + a.slice);                 // [num_bias]
+  __shared__ int s_listed;
   const int tid = threadIdx.x, lane = tid & 31;
   const int v0 = blockIdx.x * a.slice, nv = min(a.slice, a.V - v0), id0 = a.vocab_begin + v0;
   const int row0 = blockIdx.y * a.rows_per_cta, row1 = min(row0 + a.rows_per_cta, a.R);
+
+  // The parameters of the CTA's rows, read once.
+  struct Meta {
+    int b, grammar, prompt, lo, n;
+    float rep, freq, pres;
+  };
+  __shared__ Meta s_meta[kMaxRows];
+  if (tid < row1 - row0) {
+    const int r = row0 + tid;
+    Meta m{a.request ? a.request[r] : r, -1, 0, 0, 0, 1.f, 0.f, 0.f};
+    if (a.allowed) {
+      const int g = a.allowed_index ? a.allowed_index[r] : r;
+      if (g >= 0 && g < a.allowed_rows) m.grammar = g;
+    }
+    if (m.b >= 0 && m.b < a.B) {
+      if (a.prompt) m.prompt = a.prompt[m.b];
+      if (a.repetition) m.rep = a.repetition[m.b];
+      if (a.frequency) m.freq = a.frequency[m.b];
+      if (a.presence) m.pres = a.presence[m.b];
+      if (a.drafts) {
+        m.lo = min(max(a.indptr[m.b], 0), a.R);
+        m.n = min(a.indptr[m.b + 1], a.R) - m.lo;
+      }
+    } else {
+      m.b = -1;
+    }
+    s_meta[tid] = m;
+  }
+  // A row's first pieces and its own path's token of this thread are read
+  // before they are needed.
+  struct Row {
+    const T* in;
+    T* out;
+    const uint32_t* bits;  // grammar words of the slice (slices begin at whole words)
+    int b, prompt, lo, n, head, pieces;
+    uint32_t path;  // entry of the slice, or ~0
+    bool has, made;
+    uint4 raw[kBatch];
+  };
+  auto path_entry = [&](const Row& w, int r, int j, bool& made) {
+    const bool on = a.mask ? j < 32 * a.mask_words && (a.mask[int64_t(r) * a.mask_words + (j >> 5)] >> (j & 31)) & 1
+                           : w.lo + j <= r;
+    if (!on) return ~0u;
+    made = a.positions[w.lo + j] >= w.prompt;
+    const uint32_t v = uint32_t(a.drafts[w.lo + j]) - uint32_t(id0);
+    return v < uint32_t(nv) ? v : ~0u;
+  };
+  auto fill = [&](Row& w, int p0) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int p = p0 + u * kRuleThreads + tid;
+      if (p < w.pieces) w.raw[u] = *reinterpret_cast<const uint4*>(w.in + w.head + p * VEC);
+    }
+  };
+  auto open = [&](Row& w, int r) {
+    w.in = reinterpret_cast<const T*>(a.logits) + r * a.in_stride + v0;
+    w.out = reinterpret_cast<T*>(a.out) + r * a.out_stride + v0;
+    // 16-byte pieces where input and output have one misalignment
+    const uint32_t skew = reinterpret_cast<uintptr_t>(w.in) & 15;
+    const bool wide = skew == (reinterpret_cast<uintptr_t>(w.out) & 15);
+    w.head = wide ? min(nv, int((16 - skew) & 15) / int(sizeof(T))) : nv;
+    w.pieces = (nv - w.head) / VEC;
+    fill(w, 0);
+  };
+  auto read_path = [&](Row& w, int r) {
+    const Meta& m = s_meta[r - row0];
+    w.b = m.b;
+    w.has = m.b >= 0;
+    w.prompt = m.prompt;
+    w.lo = m.lo;
+    w.n = m.n;
+    w.bits = m.grammar >= 0 ? reinterpret_cast<const uint32_t*>(a.allowed + m.grammar * a.allowed_stride) + (v0 >> 5)
+                            : nullptr;
+    w.path = ~0u;
+    w.made = false;
+    if (tid < w.n) w.path = path_entry(w, r, tid, w.made);
+  };
+
+  auto touch = [&](uint32_t v) {
+    const uint32_t bit = 1u << (v & 31);
+    if (!(atomicOr(&s_bits[v >> 5], bit) & bit)) s_list[atomicAdd(&s_listed, 1)] = uint16_t(v);
+  };
+
+  Row w;
+  open(w, row0);
+  __syncthreads();
+  read_path(w, row0);
   int counted = -1;  // request whose tokens the table holds
   for (int r = row0; r < row1; ++r) {
-    const int b = a.request ? a.request[r] : r;
-    const bool has = b >= 0 && b < a.B;
-    const int prompt = has && a.prompt ? a.prompt[b] : 0;
-    if (has && b != counted) {
+    if (w.has && w.b != counted) {
+      const int len = a.tokens ? min(a.lens[w.b], a.tokens_len) : 0;
+      const int32_t* tok = a.tokens + w.b * a.tokens_stride;
+      int32_t ahead[kAhead];
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) ahead[x] = tid + x * kRuleThreads < len ? tok[tid + x * kRuleThreads] : -1;
       for (int i = tid; i < a.slice / 4; i += kRuleThreads) reinterpret_cast<uint4*>(s_count)[i] = make_uint4(0, 0, 0, 0);
       for (int i = tid; i <= a.slice / 32; i += kRuleThreads) s_bits[i] = 0;
+      if (tid == 0) s_listed = 0;
       __syncthreads();
-      if (a.tokens) {
-        const int len = min(a.lens[b], a.tokens_len);
-        const int32_t* tok = a.tokens + b * a.tokens_stride;
-#pragma unroll 8
-        for (int i = tid; i < len; i += kRuleThreads) {
-          const uint32_t v = uint32_t(tok[i]) - uint32_t(id0);
-          if (v < uint32_t(nv)) {
-            if (i >= prompt) atomicAdd(&s_count[v], 1u);
-            else atomicOr(&s_count[v], kSeen);
-            atomicOr(&s_bits[v >> 5], 1u << (v & 31));
-          }
+      auto count = [&](int32_t id, int i) {
+        const uint32_t v = uint32_t(id) - uint32_t(id0);
+        if (id >= 0 && v < uint32_t(nv)) {
+          if (i >= w.prompt) atomicAdd(&s_count[v], 1u);
+          else atomicOr(&s_count[v], kSeen);
+          touch(v);
         }
+      };
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) count(ahead[x], tid + x * kRuleThreads);
+      for (int i0 = kAhead * kRuleThreads; i0 < len; i0 += kAhead * kRuleThreads) {
+#pragma unroll
+        for (int x = 0; x < kAhead; ++x) {
+          const int i = i0 + tid + x * kRuleThreads;
+          ahead[x] = i < len ? tok[i] : -1;
+        }
+#pragma unroll
+        for (int x = 0; x < kAhead; ++x) count(ahead[x], i0 + tid + x * kRuleThreads);
       }
       if (a.num_bias && tid < 32) {
         // in the order of the list, so that an id listed several times gets
         // the same sum every time; the first of equal ids owns the sum
         for (int i0 = 0; i0 < a.num_bias; i0 += 32) {
           const int i = i0 + lane;
-          const int id = i < a.num_bias ? a.bias_ids[b * a.bias_stride + i] : -1;
+          const int id = i < a.num_bias ? a.bias_ids[w.b * a.bias_stride + i] : -1;
           const uint32_t v = uint32_t(id) - uint32_t(id0);
           const bool in = id >= 0 && v < uint32_t(nv);
-          const float value = in ? a.bias_values[b * a.bias_value_stride + i] : 0.f;
+          const uint32_t any = __ballot_sync(0xffffffffu, in);
+          if (!any) continue;
+          const float value = in ? a.bias_values[w.b * a.bias_value_stride + i] : 0.f;
           const uint32_t same = __match_any_sync(0xffffffffu, in ? int(v) : -1 - lane);
           float sum = 0.f;
           int number = -1;
@@ -142,7 +301,7 @@ __global__ void __launch_bounds__(kRuleThreads, 2) logits_rules_kernel(const Rul
             number = int((s_count[v] & ~kSeen) >> kBiasShift) - 1;
             if (number >= 0) sum = s_bias[number];
           }
-          for (uint32_t rest = 0xffffffffu; rest; rest &= rest - 1) {
+          for (uint32_t rest = any; rest; rest &= rest - 1) {
             const int from = __ffs(rest) - 1;
             const float x = __shfl_sync(0xffffffffu, value, from);
             if ((same >> from) & 1u) sum = __fadd_rn(sum, x);
@@ -151,47 +310,34 @@ __global__ void __launch_bounds__(kRuleThreads, 2) logits_rules_kernel(const Rul
             if (number < 0) {
               number = i;
               atomicOr(&s_count[v], uint32_t(i + 1) << kBiasShift);
-              atomicOr(&s_bits[v >> 5], 1u << (v & 31));
+              touch(v);
             }
             s_bias[number] = sum;
           }
           __syncwarp();
         }
       }
-      counted = b;
+      counted = w.b;
     }
     // the row's own path
-    int lo = 0, n = 0;
-    if (has && a.drafts) {
-      lo = min(max(a.indptr[b], 0), a.R);
-      n = min(a.indptr[b + 1], a.R) - lo;
-    }
     auto path = [&](auto&& use) {
-      for (int j = tid; j < n; j += kRuleThreads) {
-        const bool on = a.mask ? j < 32 * a.mask_words && (a.mask[int64_t(r) * a.mask_words + (j >> 5)] >> (j & 31)) & 1
-                               : lo + j <= r;
-        const uint32_t v = on ? uint32_t(a.drafts[lo + j]) - uint32_t(id0) : 0xffffffffu;
-        if (v < uint32_t(nv)) use(v, a.positions[lo + j] >= prompt);
+      if (w.path != ~0u) use(w.path, w.made);
+      for (int j = tid + kRuleThreads; j < w.n; j += kRuleThreads) {
+        bool made = false;
+        const uint32_t v = path_entry(w, r, j, made);
+        if (v != ~0u) use(v, made);
       }
     };
     bool lasting = false;
     path([&](uint32_t v, bool made) {
       if (made) atomicAdd(&s_count[v], 1u);
       else lasting = true, atomicOr(&s_count[v], kSeen);
-      atomicOr(&s_bits[v >> 5], 1u << (v & 31));
+      touch(v);
     });
     if (__syncthreads_or(lasting)) counted = -1;  // a prompt token of the path stays in the table
 
-    const float rep = has && a.repetition ? a.repetition[b] : 1.f;
-    const float freq = has && a.frequency ? a.frequency[b] : 0.f;
-    const float pres = has && a.presence ? a.presence[b] : 0.f;
-    int g = -1;
-    if (a.allowed) g = a.allowed_index ? a.allowed_index[r] : r;
-    // grammar words of the slice (slices begin at whole words)
-    const uint32_t* bits =
-        g >= 0 && g < a.allowed_rows ? reinterpret_cast<const uint32_t*>(a.allowed + g * a.allowed_stride) + (v0 >> 5) : nullptr;
-    const T* in = reinterpret_cast<const T*>(a.logits) + r * a.in_stride + v0;
-    T* out = reinterpret_cast<T*>(a.out) + r * a.out_stride + v0;
+    const float rep = s_meta[r - row0].rep, freq = s_meta[r - row0].freq, pres = s_meta[r - row0].pres;
+    const uint32_t* bits = w.bits;
     auto rules = [&](float x, int i) {  // entry i of the slice, not masked
       const uint32_t c = s_count[i], count = c & kCountMask, number = (c & ~kSeen) >> kBiasShift;
       if ((c & kSeen) || count) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
@@ -199,70 +345,97 @@ __global__ void __launch_bounds__(kRuleThreads, 2) logits_rules_kernel(const Rul
       if (number) x = __fadd_rn(x, s_bias[number - 1]);
       return x;
     };
-    float top = NAN;              // largest value of the 16-byte pieces so far (NaN: none yet, or it is one)
-    unsigned long long best = 0;  // largest key so far
-    auto one = [&](int i) {
-      float x = load(in + i);
-      if (has && (s_bits[i >> 5] >> (i & 31)) & 1u) x = rules(x, i);
-      if (bits && !((bits[i >> 5] >> (i & 31)) & 1u)) x = -INFINITY;
-      const T y = round_to<T>(x);
-      out[i] = y;
-      const unsigned long long key = greedy_key(load(&y), v0 + i);
+    // largest entry of the thread's 16-byte pieces (as an ordered integer) and
+    // the first piece that has it; largest key of the other entries
+    uint32_t top = 0;
+    int top_piece = -1;
+    unsigned long long best = 0;
+    auto touched_at = [&](int i) { return w.has && (s_bits[i >> 5] >> (i & 31)) & 1u; };
+    auto free_at = [&](int i) { return !bits || (bits[i >> 5] >> (i & 31)) & 1u; };
+    auto consider = [&](float y, int i) {
+      const unsigned long long key = greedy_key(y, v0 + i);
       best = key > best ? key : best;
     };
-    // 16-byte pieces where input and output have one misalignment
-    const int skew = int((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T));
-    const bool wide = (reinterpret_cast<uintptr_t>(in) & 15) == (reinterpret_cast<uintptr_t>(out) & 15);
-    const int head = wide ? min(nv, (VEC - skew) % VEC) : nv, pieces = (nv - head) / VEC;
-    for (int i = tid; i < head; i += kRuleThreads) one(i);
-    for (int i = head + pieces * VEC + tid; i < nv; i += kRuleThreads) one(i);
-#pragma unroll 2
-    for (int p = tid; p < pieces; p += kRuleThreads) {
-      const int i = head + p * VEC, w = i >> 5;
-      uint4 raw = *reinterpret_cast<const uint4*>(in + i);
-      uint32_t touched = 0, free = ~0u;
-      if (has) touched = __funnelshift_r(s_bits[w], s_bits[w + 1], i & 31);
-      if (bits) free = __funnelshift_r(bits[w], (i & 31) + VEC > 32 ? bits[w + 1] : 0u, i & 31);
-      constexpr uint32_t kAll = (1u << VEC) - 1u;
-      T* e = reinterpret_cast<T*>(&raw);
-      if ((touched | ~free) & kAll) {
+    auto one = [&](int i) {
+      const T y = free_at(i) ? w.in[i] : round_to<T>(-INFINITY);
+      w.out[i] = y;
+      if (!touched_at(i)) consider(load(&y), i);
+    };
+    for (int p0 = 0; p0 < w.pieces; p0 += kBatch * kRuleThreads) {
+      if (p0 > 0) fill(w, p0);
+      uint32_t free[kBatch];
 #pragma unroll
-        for (int x = 0; x < VEC; ++x) {
-          if (!((free >> x) & 1u)) e[x] = round_to<T>(-INFINITY);
-          else if ((touched >> x) & 1u) e[x] = round_to<T>(rules(load(e + x), i + x));
-        }
+      for (int u = 0; u < kBatch; ++u) {
+        const int p = p0 + u * kRuleThreads + tid, i = w.head + p * VEC, at = i >> 5;
+        free[u] = ~0u;
+        if (bits && p < w.pieces)
+          free[u] = __funnelshift_r(bits[at], (i & 31) + VEC > 32 ? bits[at + 1] : 0u, i & 31);
       }
-      *reinterpret_cast<uint4*>(out + i) = raw;
-      if (a.best) {
-        float mx = load(e);
 #pragma unroll
-        for (int x = 1; x < VEC; ++x) mx = max_nan(mx, load(e + x));
-        if (!(mx <= top)) {  // larger than all before, or NaN, or the first
-          top = mx;
-#pragma unroll
-          for (int x = 0; x < VEC; ++x) {
-            const unsigned long long key = greedy_key(load(e + x), v0 + i + x);
-            best = key > best ? key : best;
+      for (int u = 0; u < kBatch; ++u) {
+        const int p = p0 + u * kRuleThreads + tid, i = w.head + p * VEC, at = i >> 5;
+        if (p >= w.pieces) continue;
+        if (bits) w.raw[u] = Pack<T>::keep(w.raw[u], free[u]);
+        *reinterpret_cast<uint4*>(w.out + i) = w.raw[u];
+        if (a.best) {
+          // Listed entries count as -inf here; their own value comes in the
+          // second pass and is no smaller.
+          uint4 x = w.raw[u];
+          if (w.has) {
+            const uint32_t listed = __funnelshift_r(s_bits[at], s_bits[at + 1], i & 31);
+            if (listed & ((1u << VEC) - 1u)) x = Pack<T>::keep(x, ~listed);
+          }
+          const uint32_t o = order_of(Pack<T>::largest(x));
+          if (o > top) {
+            top = o;
+            top_piece = p;
           }
         }
       }
     }
-    if (a.best) {
-#pragma unroll
-      for (int m = 16; m > 0; m >>= 1) {
-        const unsigned long long o = __shfl_xor_sync(0xffffffffu, best, m);
-        best = o > best ? o : best;
+    for (int i = tid; i < w.head; i += kRuleThreads) one(i);
+    for (int i = w.head + w.pieces * VEC + tid; i < nv; i += kRuleThreads) one(i);
+    if (w.has) {
+      // The stream left listed entries as they were (or -inf), so they can be
+      // read back also where the output is the input.
+      __syncthreads();
+      const int listed = s_listed;
+#pragma unroll 2
+      for (int j = tid; j < listed; j += kRuleThreads) {
+        const int i = s_list[j];
+        T y = round_to<T>(-INFINITY);
+        if (free_at(i)) {
+          y = round_to<T>(rules(load(w.in + i), i));
+          w.out[i] = y;
+        }
+        consider(load(&y), i);
       }
+    }
+    if (a.best) {
+      // where in the piece: only the lanes that hold the warp's largest entry
+      const uint32_t highest = __reduce_max_sync(0xffffffffu, top);
+      if (top_piece >= 0 && top == highest) {
+        const int i = w.head + top_piece * VEC;
+        for (int x = 0; x < VEC; ++x) {
+          const T y = w.out[i + x];
+          consider(touched_at(i + x) ? -INFINITY : load(&y), i + x);
+        }
+      }
+      __syncwarp();
+      best = warp_max(best);
       if (lane == 0) s_best[tid >> 5] = best;
     }
     __syncthreads();
-    if (a.best && tid == 0) {
-      for (int w = 1; w < kRuleThreads / 32; ++w) best = s_best[w] > best ? s_best[w] : best;
-      a.best[int64_t(r) * a.slices + blockIdx.x] = best;
+    if (a.best && tid < 32) {
+      best = warp_max(lane < kRuleThreads / 32 ? s_best[lane] : 0ull);
+      if (tid == 0) a.best[int64_t(r) * a.slices + blockIdx.x] = best;
     }
-    if (counted >= 0 && r + 1 < row1)
-      path([&](uint32_t v, bool) { atomicSub(&s_count[v], 1u); });
-    __syncthreads();
+    if (r + 1 < row1) {
+      if (counted >= 0) path([&](uint32_t v, bool) { atomicSub(&s_count[v], 1u); });
+      open(w, r + 1);
+      read_path(w, r + 1);
+      __syncthreads();
+    }
   }
 }
 
@@ -418,7 +591,7 @@ void process_logits(torch::Tensor logits, torch::Tensor out, c10::optional<torch
   // Rows of a CTA share one count of their request's tokens, and a wide slice
   // reads the tokens less often (16384 entries: 8 to 10 times a row); but
   // first the GPU's 2 x 148 places have to be filled.
-  int64_t slice = kMaxSlice, rows = 8;
+  int64_t slice = kMaxSlice, rows = kMaxRows;
   auto ctas = [&] { return ((V + slice - 1) / slice) * ((R + rows - 1) / rows); };
   while (rows > 1 && ctas() < 2 * 2 * kNumSMs) rows /= 2;
   while (slice > kMinSlice && ctas() < 2 * kNumSMs) slice /= 2;
@@ -426,7 +599,7 @@ void process_logits(torch::Tensor logits, torch::Tensor out, c10::optional<torch
   a.slices = int((V + slice - 1) / slice);
   a.rows_per_cta = int(rows);
   const dim3 grid{unsigned(a.slices), unsigned((R + rows - 1) / rows)};
-  const size_t smem = size_t(slice + slice / 32 + 1 + a.num_bias) * 4;
+  const size_t smem = size_t(slice + slice / 32 + 4 + slice / 2 + a.num_bias) * 4;
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
   torch::Tensor best;
   if (greedy.has_value()) {

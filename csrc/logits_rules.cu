@@ -9,15 +9,16 @@
 // end of its prompt) and over the drafted tokens on the row's own tree path.
 //
 // Every logit is read and written once: bound by HBM for many rows, by
-// latency for one.  A CTA takes a slice of the vocabulary for a few rows: it
-// counts the request's tokens that fall into the slice in shared memory (a
-// word an entry, integer atomics, so the order does not matter), once for all
-// rows of a request, and lists the entries that any rule touches.  A row then
-// streams through 16-byte loads and stores with the grammar bits alone, and
-// the listed entries are computed in a second, short pass: with the rules in
-// the stream, a warp took their branches for nearly every piece (512 rows of
-// fp32: 255 us).  A row's path tokens are added before it and taken back
-// after it.
+// latency for one.  A CTA takes a slice of the vocabulary for a few rows.  For
+// each run of rows of one request it counts the request's tokens that fall
+// into the slice in shared memory (a word an entry, integer atomics, so the
+// order does not matter) and lists the entries that any rule touches, the
+// request's drafted tokens among them.  Then its warps go their own ways, a
+// row or a part of one each: a stream of 16-byte loads and stores that knows
+// only the grammar bits, then the listed entries, where a drafted token's
+// count adds those on the row's own path.  With the rules inside the stream a
+// warp took their branches for nearly every piece, and with the block on one
+// row at a time it waited at barriers (8 trees of 32, V = 152064: 82 us).
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -29,14 +30,16 @@ namespace kvs {
 namespace {
 
 constexpr int kRuleThreads = 512;
+constexpr int kRuleWarps = kRuleThreads / 32;
 constexpr int kMaxSlice = 16384;  // entries: 64 KB of counts and 32 KB of list, two CTAs on an SM
 constexpr int kMinSlice = 1024;
 constexpr int kMaxBias = 2047;
-// a count word: bit 31 seen in the prompt, bits 20..30 bias number + 1, then
-// the count of generated occurrences
+// a count word: bit 31 seen in the prompt, bits 20..30 bias number + 1, bit 19
+// drafted, then the count of generated occurrences
 constexpr uint32_t kSeen = 0x80000000u;
 constexpr int kBiasShift = 20;
-constexpr uint32_t kCountMask = (1u << kBiasShift) - 1u;
+constexpr uint32_t kDrafted = 1u << 19;
+constexpr uint32_t kCountMask = kDrafted - 1u;
 
 struct RuleArgs {
   const void* logits;
@@ -148,126 +151,61 @@ __device__ __forceinline__ unsigned long long warp_max(unsigned long long k) {
 }
 
 constexpr int kMaxRows = 8;   // rows of a CTA
-constexpr int kBatch = 4;  // 16-byte pieces of a thread in flight
-constexpr int kAhead = 8;  // tokens of a thread read while the table is cleared
+constexpr int kBatch = 4;     // 16-byte pieces of a lane in flight
+constexpr int kAhead = 8;     // tokens of a thread read while the table is cleared
+constexpr int kPartPieces = 64;  // pieces of a warp's part of a row, at least
 
 template <typename T>
 __global__ void __launch_bounds__(kRuleThreads, 2) logits_rules_kernel(const RuleArgs a) {
   pdl_trigger();
   constexpr int VEC = 16 / sizeof(T);
   extern __shared__ uint32_t sm[];
-  __shared__ unsigned long long s_best[kRuleThreads / 32];
   uint32_t* s_count = sm;                     // [slice]
   uint32_t* s_bits = s_count + a.slice;       // [slice / 32 + 4] entries that a rule may change ...
   uint16_t* s_list = reinterpret_cast<uint16_t*>(s_bits + a.slice / 32 + 4);  // [slice] ... and their list
   float* s_bias = reinterpret_cast<float*>(s_list + a.slice);                 // [num_bias]
   __shared__ int s_listed;
-  const int tid = threadIdx.x, lane = tid & 31;
+  __shared__ unsigned long long s_best[kMaxRows];
+  __shared__ int s_request[kMaxRows];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int v0 = blockIdx.x * a.slice, nv = min(a.slice, a.V - v0), id0 = a.vocab_begin + v0;
   const int row0 = blockIdx.y * a.rows_per_cta, row1 = min(row0 + a.rows_per_cta, a.R);
-
-  // The parameters of the CTA's rows, read once.
-  struct Meta {
-    int b, grammar, prompt, lo, n;
-    float rep, freq, pres;
-  };
-  __shared__ Meta s_meta[kMaxRows];
   if (tid < row1 - row0) {
-    const int r = row0 + tid;
-    Meta m{a.request ? a.request[r] : r, -1, 0, 0, 0, 1.f, 0.f, 0.f};
-    if (a.allowed) {
-      const int g = a.allowed_index ? a.allowed_index[r] : r;
-      if (g >= 0 && g < a.allowed_rows) m.grammar = g;
-    }
-    if (m.b >= 0 && m.b < a.B) {
-      if (a.prompt) m.prompt = a.prompt[m.b];
-      if (a.repetition) m.rep = a.repetition[m.b];
-      if (a.frequency) m.freq = a.frequency[m.b];
-      if (a.presence) m.pres = a.presence[m.b];
-      if (a.drafts) {
-        m.lo = min(max(a.indptr[m.b], 0), a.R);
-        m.n = min(a.indptr[m.b + 1], a.R) - m.lo;
-      }
-    } else {
-      m.b = -1;
-    }
-    s_meta[tid] = m;
+    const int b = a.request ? a.request[row0 + tid] : row0 + tid;
+    s_request[tid] = b >= 0 && b < a.B ? b : -1;
   }
-  // A row's first pieces and its own path's token of this thread are read
-  // before they are needed.
-  struct Row {
-    const T* in;
-    T* out;
-    const uint32_t* bits;  // grammar words of the slice (slices begin at whole words)
-    int b, prompt, lo, n, head, pieces;
-    uint32_t path;  // entry of the slice, or ~0
-    bool has, made;
-    uint4 raw[kBatch];
-  };
-  auto path_entry = [&](const Row& w, int r, int j, bool& made) {
-    const bool on = a.mask ? j < 32 * a.mask_words && (a.mask[int64_t(r) * a.mask_words + (j >> 5)] >> (j & 31)) & 1
-                           : w.lo + j <= r;
-    if (!on) return ~0u;
-    made = a.positions[w.lo + j] >= w.prompt;
-    const uint32_t v = uint32_t(a.drafts[w.lo + j]) - uint32_t(id0);
-    return v < uint32_t(nv) ? v : ~0u;
-  };
-  auto fill = [&](Row& w, int p0) {
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int p = p0 + u * kRuleThreads + tid;
-      if (p < w.pieces) w.raw[u] = *reinterpret_cast<const uint4*>(w.in + w.head + p * VEC);
-    }
-  };
-  auto open = [&](Row& w, int r) {
-    w.in = reinterpret_cast<const T*>(a.logits) + r * a.in_stride + v0;
-    w.out = reinterpret_cast<T*>(a.out) + r * a.out_stride + v0;
-    // 16-byte pieces where input and output have one misalignment
-    const uint32_t skew = reinterpret_cast<uintptr_t>(w.in) & 15;
-    const bool wide = skew == (reinterpret_cast<uintptr_t>(w.out) & 15);
-    w.head = wide ? min(nv, int((16 - skew) & 15) / int(sizeof(T))) : nv;
-    w.pieces = (nv - w.head) / VEC;
-    fill(w, 0);
-  };
-  auto read_path = [&](Row& w, int r) {
-    const Meta& m = s_meta[r - row0];
-    w.b = m.b;
-    w.has = m.b >= 0;
-    w.prompt = m.prompt;
-    w.lo = m.lo;
-    w.n = m.n;
-    w.bits = m.grammar >= 0 ? reinterpret_cast<const uint32_t*>(a.allowed + m.grammar * a.allowed_stride) + (v0 >> 5)
-                            : nullptr;
-    w.path = ~0u;
-    w.made = false;
-    if (tid < w.n) w.path = path_entry(w, r, tid, w.made);
-  };
-
+  __syncthreads();
   auto touch = [&](uint32_t v) {
     const uint32_t bit = 1u << (v & 31);
     if (!(atomicOr(&s_bits[v >> 5], bit) & bit)) s_list[atomicAdd(&s_listed, 1)] = uint16_t(v);
   };
 
-  Row w;
-  open(w, row0);
-  __syncthreads();
-  read_path(w, row0);
-  int counted = -1;  // request whose tokens the table holds
-  for (int r = row0; r < row1; ++r) {
-    if (w.has && w.b != counted) {
-      const int len = a.tokens ? min(a.lens[w.b], a.tokens_len) : 0;
-      const int32_t* tok = a.tokens + w.b * a.tokens_stride;
+  for (int r0 = row0; r0 < row1;) {
+    const int b = s_request[r0 - row0];
+    int run = 1;
+    while (r0 + run < row1 && s_request[r0 + run - row0] == b) ++run;
+    const bool has = b >= 0;
+    const int prompt = has && a.prompt ? a.prompt[b] : 0;
+    int lo = 0, n = 0;
+    if (tid < kMaxRows) s_best[tid] = 0;
+    if (tid == 0) s_listed = 0;
+    if (has) {
+      const int len = a.tokens ? min(a.lens[b], a.tokens_len) : 0;
+      const int32_t* tok = a.tokens + b * a.tokens_stride;
       int32_t ahead[kAhead];
 #pragma unroll
       for (int x = 0; x < kAhead; ++x) ahead[x] = tid + x * kRuleThreads < len ? tok[tid + x * kRuleThreads] : -1;
+      if (a.drafts) {
+        lo = min(max(a.indptr[b], 0), a.R);
+        n = min(a.indptr[b + 1], a.R) - lo;
+      }
       for (int i = tid; i < a.slice / 4; i += kRuleThreads) reinterpret_cast<uint4*>(s_count)[i] = make_uint4(0, 0, 0, 0);
       for (int i = tid; i <= a.slice / 32; i += kRuleThreads) s_bits[i] = 0;
-      if (tid == 0) s_listed = 0;
       __syncthreads();
       auto count = [&](int32_t id, int i) {
         const uint32_t v = uint32_t(id) - uint32_t(id0);
         if (id >= 0 && v < uint32_t(nv)) {
-          if (i >= w.prompt) atomicAdd(&s_count[v], 1u);
+          if (i >= prompt) atomicAdd(&s_count[v], 1u);
           else atomicOr(&s_count[v], kSeen);
           touch(v);
         }
@@ -283,17 +221,25 @@ __global__ void __launch_bounds__(kRuleThreads, 2) logits_rules_kernel(const Rul
 #pragma unroll
         for (int x = 0; x < kAhead; ++x) count(ahead[x], i0 + tid + x * kRuleThreads);
       }
-      if (a.num_bias && tid < 32) {
+      for (int j = tid; j < n; j += kRuleThreads) {
+        const int32_t id = a.drafts[lo + j];
+        const uint32_t v = uint32_t(id) - uint32_t(id0);
+        if (id >= 0 && v < uint32_t(nv)) {
+          atomicOr(&s_count[v], kDrafted);
+          touch(v);
+        }
+      }
+      if (a.num_bias && warp == kRuleWarps - 1) {
         // in the order of the list, so that an id listed several times gets
         // the same sum every time; the first of equal ids owns the sum
         for (int i0 = 0; i0 < a.num_bias; i0 += 32) {
           const int i = i0 + lane;
-          const int id = i < a.num_bias ? a.bias_ids[w.b * a.bias_stride + i] : -1;
+          const int id = i < a.num_bias ? a.bias_ids[b * a.bias_stride + i] : -1;
           const uint32_t v = uint32_t(id) - uint32_t(id0);
           const bool in = id >= 0 && v < uint32_t(nv);
           const uint32_t any = __ballot_sync(0xffffffffu, in);
           if (!any) continue;
-          const float value = in ? a.bias_values[w.b * a.bias_value_stride + i] : 0.f;
+          const float value = in ? a.bias_values[b * a.bias_value_stride + i] : 0.f;
           const uint32_t same = __match_any_sync(0xffffffffu, in ? int(v) : -1 - lane);
           float sum = 0.f;
           int number = -1;
@@ -317,125 +263,134 @@ __global__ void __launch_bounds__(kRuleThreads, 2) logits_rules_kernel(const Rul
           __syncwarp();
         }
       }
-      counted = w.b;
-    }
-    // the row's own path
-    auto path = [&](auto&& use) {
-      if (w.path != ~0u) use(w.path, w.made);
-      for (int j = tid + kRuleThreads; j < w.n; j += kRuleThreads) {
-        bool made = false;
-        const uint32_t v = path_entry(w, r, j, made);
-        if (v != ~0u) use(v, made);
-      }
-    };
-    bool lasting = false;
-    path([&](uint32_t v, bool made) {
-      if (made) atomicAdd(&s_count[v], 1u);
-      else lasting = true, atomicOr(&s_count[v], kSeen);
-      touch(v);
-    });
-    if (__syncthreads_or(lasting)) counted = -1;  // a prompt token of the path stays in the table
-
-    const float rep = s_meta[r - row0].rep, freq = s_meta[r - row0].freq, pres = s_meta[r - row0].pres;
-    const uint32_t* bits = w.bits;
-    auto rules = [&](float x, int i) {  // entry i of the slice, not masked
-      const uint32_t c = s_count[i], count = c & kCountMask, number = (c & ~kSeen) >> kBiasShift;
-      if ((c & kSeen) || count) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-      if (count) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, float(count))), pres);
-      if (number) x = __fadd_rn(x, s_bias[number - 1]);
-      return x;
-    };
-    // largest entry of the thread's 16-byte pieces (as an ordered integer) and
-    // the first piece that has it; largest key of the other entries
-    uint32_t top = 0;
-    int top_piece = -1;
-    unsigned long long best = 0;
-    auto touched_at = [&](int i) { return w.has && (s_bits[i >> 5] >> (i & 31)) & 1u; };
-    auto free_at = [&](int i) { return !bits || (bits[i >> 5] >> (i & 31)) & 1u; };
-    auto consider = [&](float y, int i) {
-      const unsigned long long key = greedy_key(y, v0 + i);
-      best = key > best ? key : best;
-    };
-    auto one = [&](int i) {
-      const T y = free_at(i) ? w.in[i] : round_to<T>(-INFINITY);
-      w.out[i] = y;
-      if (!touched_at(i)) consider(load(&y), i);
-    };
-    for (int p0 = 0; p0 < w.pieces; p0 += kBatch * kRuleThreads) {
-      if (p0 > 0) fill(w, p0);
-      uint32_t free[kBatch];
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const int p = p0 + u * kRuleThreads + tid, i = w.head + p * VEC, at = i >> 5;
-        free[u] = ~0u;
-        if (bits && p < w.pieces)
-          free[u] = __funnelshift_r(bits[at], (i & 31) + VEC > 32 ? bits[at + 1] : 0u, i & 31);
-      }
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const int p = p0 + u * kRuleThreads + tid, i = w.head + p * VEC, at = i >> 5;
-        if (p >= w.pieces) continue;
-        if (bits) w.raw[u] = Pack<T>::keep(w.raw[u], free[u]);
-        *reinterpret_cast<uint4*>(w.out + i) = w.raw[u];
-        if (a.best) {
-          // Listed entries count as -inf here; their own value comes in the
-          // second pass and is no smaller.
-          uint4 x = w.raw[u];
-          if (w.has) {
-            const uint32_t listed = __funnelshift_r(s_bits[at], s_bits[at + 1], i & 31);
-            if (listed & ((1u << VEC) - 1u)) x = Pack<T>::keep(x, ~listed);
-          }
-          const uint32_t o = order_of(Pack<T>::largest(x));
-          if (o > top) {
-            top = o;
-            top_piece = p;
-          }
-        }
-      }
-    }
-    for (int i = tid; i < w.head; i += kRuleThreads) one(i);
-    for (int i = w.head + w.pieces * VEC + tid; i < nv; i += kRuleThreads) one(i);
-    if (w.has) {
-      // The stream left listed entries as they were (or -inf), so they can be
-      // read back also where the output is the input.
-      __syncthreads();
-      const int listed = s_listed;
-#pragma unroll 2
-      for (int j = tid; j < listed; j += kRuleThreads) {
-        const int i = s_list[j];
-        T y = round_to<T>(-INFINITY);
-        if (free_at(i)) {
-          y = round_to<T>(rules(load(w.in + i), i));
-          w.out[i] = y;
-        }
-        consider(load(&y), i);
-      }
-    }
-    if (a.best) {
-      // where in the piece: only the lanes that hold the warp's largest entry
-      const uint32_t highest = __reduce_max_sync(0xffffffffu, top);
-      if (top_piece >= 0 && top == highest) {
-        const int i = w.head + top_piece * VEC;
-        for (int x = 0; x < VEC; ++x) {
-          const T y = w.out[i + x];
-          consider(touched_at(i + x) ? -INFINITY : load(&y), i + x);
-        }
-      }
-      __syncwarp();
-      best = warp_max(best);
-      if (lane == 0) s_best[tid >> 5] = best;
     }
     __syncthreads();
-    if (a.best && tid < 32) {
-      best = warp_max(lane < kRuleThreads / 32 ? s_best[lane] : 0ull);
-      if (tid == 0) a.best[int64_t(r) * a.slices + blockIdx.x] = best;
+
+    // one row, or a part of one, to each warp
+    const int row_parts = kRuleWarps / run, x = warp / row_parts, part = warp % row_parts, r = r0 + x;
+    const T* in = reinterpret_cast<const T*>(a.logits) + r * a.in_stride + v0;
+    T* out = reinterpret_cast<T*>(a.out) + r * a.out_stride + v0;
+    // 16-byte pieces where input and output have one misalignment
+    const uint32_t skew = reinterpret_cast<uintptr_t>(in) & 15;
+    const bool wide = skew == (reinterpret_cast<uintptr_t>(out) & 15);
+    const int head = wide ? min(nv, int((16 - skew) & 15) / int(sizeof(T))) : nv, pieces = (nv - head) / VEC;
+    const int parts = wide ? max(1, min(row_parts, (pieces + kPartPieces - 1) / kPartPieces)) : row_parts;
+    if (x < run && part < parts) {
+      int g = -1;
+      if (a.allowed) g = a.allowed_index ? a.allowed_index[r] : r;
+      // grammar words of the slice (slices begin at whole words)
+      const uint32_t* bits = g >= 0 && g < a.allowed_rows
+                                 ? reinterpret_cast<const uint32_t*>(a.allowed + g * a.allowed_stride) + (v0 >> 5)
+                                 : nullptr;
+      // largest entry of the lane's 16-byte pieces (as an ordered integer) and
+      // the first piece that has it; largest key of the other entries
+      uint32_t top = 0;
+      int top_piece = -1;
+      unsigned long long best = 0;
+      auto touched_at = [&](int i) { return has && (s_bits[i >> 5] >> (i & 31)) & 1u; };
+      auto free_at = [&](int i) { return !bits || (bits[i >> 5] >> (i & 31)) & 1u; };
+      auto consider = [&](float y, int i) {
+        const unsigned long long key = greedy_key(y, v0 + i);
+        best = key > best ? key : best;
+      };
+      const int per = (pieces + parts - 1) / parts, p_end = min(pieces, (part + 1) * per);
+      for (int p0 = part * per; p0 < p_end; p0 += 32 * kBatch) {
+        uint4 raw[kBatch];
+        uint32_t free[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int p = p0 + u * 32 + lane, i = head + p * VEC, at = i >> 5;
+          free[u] = ~0u;
+          if (p < p_end) {
+            raw[u] = *reinterpret_cast<const uint4*>(in + i);
+            if (bits) free[u] = __funnelshift_r(bits[at], (i & 31) + VEC > 32 ? bits[at + 1] : 0u, i & 31);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int p = p0 + u * 32 + lane, i = head + p * VEC, at = i >> 5;
+          if (p >= p_end) continue;
+          if (bits) raw[u] = Pack<T>::keep(raw[u], free[u]);
+          *reinterpret_cast<uint4*>(out + i) = raw[u];
+          if (a.best) {
+            // Listed entries count as -inf here; their own value comes in the
+            // second pass and is no smaller.
+            if (has) {
+              const uint32_t listed = __funnelshift_r(s_bits[at], s_bits[at + 1], i & 31);
+              if (listed & ((1u << VEC) - 1u)) raw[u] = Pack<T>::keep(raw[u], ~listed);
+            }
+            const uint32_t o = order_of(Pack<T>::largest(raw[u]));
+            if (o > top) {
+              top = o;
+              top_piece = p;
+            }
+          }
+        }
+      }
+      auto one = [&](int i) {
+        const T y = free_at(i) ? in[i] : round_to<T>(-INFINITY);
+        out[i] = y;
+        if (!touched_at(i)) consider(load(&y), i);
+      };
+      const int at = part * 32 + lane, step = parts * 32;
+      for (int i = at; i < head; i += step) one(i);
+      for (int i = head + pieces * VEC + at; i < nv; i += step) one(i);
+      if (has) {
+        // The stream left listed entries as they were (or -inf), so they can
+        // be read back also where the output is the input.
+        __syncwarp();
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + x), "r"(parts * 32) : "memory");
+        const float rep = a.repetition ? a.repetition[b] : 1.f;
+        const float freq = a.frequency ? a.frequency[b] : 0.f;
+        const float pres = a.presence ? a.presence[b] : 0.f;
+        const int listed = s_listed;
+        for (int j = at; j < listed; j += step) {
+          const int i = s_list[j];
+          T y = round_to<T>(-INFINITY);
+          if (free_at(i)) {
+            float v = load(in + i);
+            const uint32_t c = s_count[i], number = (c & ~kSeen) >> kBiasShift;
+            uint32_t times = c & kCountMask;
+            bool seen = c & kSeen;
+            if (c & kDrafted) {  // on the row's own path
+              for (int k = 0; k < n; ++k) {
+                const bool on = a.mask ? k < 32 * a.mask_words &&
+                                             (a.mask[int64_t(r) * a.mask_words + (k >> 5)] >> (k & 31)) & 1
+                                       : lo + k <= r;
+                if (!on || a.drafts[lo + k] != id0 + i) continue;
+                if (a.positions[lo + k] >= prompt) ++times;
+                else seen = true;
+              }
+            }
+            if (seen || times) v = v > 0.f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
+            if (times) v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, float(times))), pres);
+            if (number) v = __fadd_rn(v, s_bias[number - 1]);
+            y = round_to<T>(v);
+            out[i] = y;
+          }
+          consider(load(&y), i);
+        }
+      }
+      if (a.best) {
+        // where in the piece: only the lanes that hold the warp's largest entry
+        __syncwarp();
+        const uint32_t highest = __reduce_max_sync(0xffffffffu, top);
+        if (top_piece >= 0 && top == highest) {
+          const int i = head + top_piece * VEC;
+          for (int e = 0; e < VEC; ++e) {
+            const T y = out[i + e];
+            consider(touched_at(i + e) ? -INFINITY : load(&y), i + e);
+          }
+        }
+        __syncwarp();
+        best = warp_max(best);
+        if (lane == 0) atomicMax(&s_best[x], best);
+      }
     }
-    if (r + 1 < row1) {
-      if (counted >= 0) path([&](uint32_t v, bool) { atomicSub(&s_count[v], 1u); });
-      open(w, r + 1);
-      read_path(w, r + 1);
-      __syncthreads();
-    }
+    __syncthreads();
+    if (a.best && tid < run) a.best[int64_t(r0 + tid) * a.slices + blockIdx.x] = s_best[tid];
+    r0 += run;
+    if (r0 < row1) __syncthreads();
   }
 }
 
@@ -593,7 +548,7 @@ void process_logits(torch::Tensor logits, torch::Tensor out, c10::optional<torch
   // first the GPU's 2 x 148 places have to be filled.
   int64_t slice = kMaxSlice, rows = kMaxRows;
   auto ctas = [&] { return ((V + slice - 1) / slice) * ((R + rows - 1) / rows); };
-  while (rows > 1 && ctas() < 2 * 2 * kNumSMs) rows /= 2;
+  while (rows > 1 && (rows > (R + B - 1) / B || ctas() < 2 * 2 * kNumSMs)) rows /= 2;
   while (slice > kMinSlice && ctas() < 2 * kNumSMs) slice /= 2;
   a.slice = int(slice);
   a.slices = int((V + slice - 1) / slice);

@@ -269,18 +269,40 @@ const int32_t* ints(const torch::Tensor& t) { return t.data_ptr<int32_t>(); }
 
 }  // namespace
 
-void plan_step(torch::Tensor ctx_lens, torch::Tensor new_lens, torch::Tensor block_tables, torch::Tensor held,
-               torch::Tensor free_queue, torch::Tensor cursor, int64_t block_size,
-               c10::optional<torch::Tensor> parents, torch::Tensor indptr, torch::Tensor row_request,
-               torch::Tensor positions, torch::Tensor slot_mapping, c10::optional<torch::Tensor> tree_mask,
-               torch::Tensor held_out, torch::Tensor cursor_out, torch::Tensor status) {
-  const int64_t B = ctx_lens.numel(), R = row_request.numel();
-  for (const torch::Tensor* t : {&ctx_lens, &new_lens, &held, &free_queue, &indptr, &row_request, &positions,
-                                 &slot_mapping, &held_out})
+std::vector<torch::Tensor> plan_step(torch::Tensor ctx_lens, torch::Tensor new_lens, torch::Tensor block_tables,
+                                     torch::Tensor held, torch::Tensor free_queue, torch::Tensor cursor,
+                                     int64_t block_size, int64_t num_rows, c10::optional<torch::Tensor> parents,
+                                     int64_t max_tree, std::vector<torch::Tensor> out, torch::Tensor status) {
+  const int64_t B = ctx_lens.numel(), R = num_rows;
+  KVS_CHECK_ARG(ctx_lens.is_cuda() && ctx_lens.scalar_type() == at::kInt, "plan_step: ctx_lens int32 on a CUDA device");
+  KVS_CHECK_ARG(R >= 0 && R < (int64_t(1) << 30), "plan_step: too many rows");
+  KVS_CHECK_ARG(max_tree >= 1 && max_tree <= 32768, "plan_step: max_tree must be 1 to 32768");
+  const int64_t words = parents.has_value() ? (max_tree + 31) / 32 : 0;
+  if (out.empty()) {
+    // one piece of memory for all outputs
+    const torch::Tensor all = torch::empty({2 * B + 1 + R * (3 + words)}, ctx_lens.options());
+    int64_t at = 0;
+    auto take = [&](int64_t n) {
+      at += n;
+      return all.narrow(0, at - n, n);
+    };
+    out = {take(B + 1), take(R), take(R), take(R)};
+    if (words) out.push_back(take(R * words).view({R, words}));
+    out.push_back(take(B));
+    out.push_back(torch::empty({2}, cursor.options()));
+  }
+  KVS_CHECK_ARG(out.size() == (words ? 7u : 6u), "plan_step: out was made for a step with other parents");
+  const torch::Tensor &indptr = out[0], &row_request = out[1], &positions = out[2], &slot_mapping = out[3],
+                      &held_out = out[out.size() - 2], &cursor_out = out[out.size() - 1];
+  c10::optional<torch::Tensor> tree_mask;
+  if (words) tree_mask = out[4];
+  KVS_CHECK_ARG(row_request.numel() == R, "plan_step: out was made for another number of rows");
+  for (const torch::Tensor* t : std::initializer_list<const torch::Tensor*>{
+           &ctx_lens, &new_lens, &held, &free_queue, &indptr, &row_request, &positions, &slot_mapping, &held_out})
     KVS_CHECK_ARG(t->is_cuda() && t->dim() == 1 && t->is_contiguous() && t->scalar_type() == at::kInt &&
                       t->device() == ctx_lens.device(),
                   "plan_step: lengths, queue and row tensors are contiguous int32 vectors on one CUDA device");
-  for (const torch::Tensor* t : {&cursor, &cursor_out})
+  for (const torch::Tensor* t : std::initializer_list<const torch::Tensor*>{&cursor, &cursor_out})
     KVS_CHECK_ARG(t->is_cuda() && t->is_contiguous() && t->scalar_type() == at::kLong && t->numel() == 2 &&
                       t->device() == ctx_lens.device(),
                   "plan_step: cursor is int64 [2] on the same device");
@@ -296,8 +318,6 @@ void plan_step(torch::Tensor ctx_lens, torch::Tensor new_lens, torch::Tensor blo
   KVS_CHECK_ARG(free_queue.numel() >= 1 && free_queue.numel() < (int64_t(1) << 30), "plan_step: free_queue size");
   KVS_CHECK_ARG(block_size >= 1 && block_size * free_queue.numel() <= INT32_MAX,
                 "plan_step: slots (blocks x block_size) must fit in 32 bits");
-  KVS_CHECK_ARG(R < (int64_t(1) << 30), "plan_step: too many rows");
-  KVS_CHECK_ARG(parents.has_value() == tree_mask.has_value(), "plan_step: tree_mask goes with parents");
   PlanArgs a{};
   if (parents.has_value()) {
     KVS_CHECK_ARG(parents->is_cuda() && parents->scalar_type() == at::kInt && parents->dim() == 1 &&
@@ -344,6 +364,7 @@ void plan_step(torch::Tensor ctx_lens, torch::Tensor new_lens, torch::Tensor blo
   step_plan_kernel<<<ctas, kPlanThreads, smem, st>>>(a);
   KVS_CUDA_CHECK(cudaGetLastError());
   if (ctas > 1) launch_pdl(step_state_kernel, dim3(unsigned((B + 255) / 256)), dim3(256), 0, st, a);
+  return out;
 }
 
 }  // namespace kvs

@@ -99,34 +99,51 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const Commi
       for (int r = min(max(a.indptr[gridDim.y], 0), a.R) + tid; r < a.R; r += kCommitThreads) a.path[r] = -1;
   }
   if (a.src == nullptr) return;
-  // a warp copies one row of one plane at a time
+  // 16-byte words of all rows and planes, four in flight a thread
   const int first = blockIdx.x * a.planes_per_cta, count = min(a.planes_per_cta, a.planes - first);
-  const int row = a.heads * a.words;
-  for (int x = warp; x < count * len; x += kCommitThreads / 32) {
-    const int plane = first + x / len, k = x % len, slot = s_slot[k];
-    if (slot < 0 || slot >= a.num_slots) {
-      if (lane == 0) atomicCAS(a.status, 0u, uint32_t(kStatusBadSize));
-      continue;
+  const int row = a.heads * a.words, total = count * len * row;
+  for (int e0 = tid; e0 < total; e0 += 4 * kCommitThreads) {
+    uint4 v[4];
+    uint4* to[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int e = e0 + u * kCommitThreads;
+      to[u] = nullptr;
+      if (e < total) {
+        const int x = e / row, c = e - x * row, plane = first + x / len, k = x % len, h = c / a.words, w = c - h * a.words;
+        const int slot = s_slot[k];
+        if (slot >= 0 && slot < a.num_slots) {
+          v[u] = a.src[(plane >> 1) * a.src_l + (plane & 1) * a.src_p + (lo + s_path[k]) * a.src_r + h * a.src_h + w];
+          to[u] = a.dst + (plane >> 1) * a.dst_l + (plane & 1) * a.dst_p + (slot / a.bs) * a.dst_b +
+                  (slot % a.bs) * a.dst_t + h * a.dst_h + w;
+        } else if (c == 0) {
+          atomicCAS(a.status, 0u, uint32_t(kStatusBadSize));
+        }
+      }
     }
-    const uint4* src = a.src + (plane >> 1) * a.src_l + (plane & 1) * a.src_p + (lo + s_path[k]) * a.src_r;
-    uint4* dst = a.dst + (plane >> 1) * a.dst_l + (plane & 1) * a.dst_p + (slot / a.bs) * a.dst_b +
-                 (slot % a.bs) * a.dst_t;
-#pragma unroll 4
-    for (int c = lane; c < row; c += 32) {
-      const int h = c / a.words, w = c - h * a.words;
-      dst[h * a.dst_h + w] = src[h * a.src_h + w];
-    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (to[u]) *to[u] = v[u];
   }
 }
 
 }  // namespace
 
-void commit_tree(torch::Tensor draft_ids, torch::Tensor target_ids, c10::optional<torch::Tensor> parents,
-                 torch::Tensor indptr, torch::Tensor ctx_lens, torch::Tensor slot_mapping,
-                 c10::optional<torch::Tensor> tree_kv, c10::optional<torch::Tensor> kv_cache,
-                 c10::optional<torch::Tensor> tokens, torch::Tensor accepted, torch::Tensor path,
-                 torch::Tensor next_ids, torch::Tensor ctx_out, torch::Tensor status) {
+std::vector<torch::Tensor> commit_tree(torch::Tensor draft_ids, torch::Tensor target_ids,
+                                       c10::optional<torch::Tensor> parents, torch::Tensor indptr,
+                                       torch::Tensor ctx_lens, torch::Tensor slot_mapping,
+                                       c10::optional<torch::Tensor> tree_kv, c10::optional<torch::Tensor> kv_cache,
+                                       c10::optional<torch::Tensor> tokens, std::vector<torch::Tensor> out,
+                                       torch::Tensor status) {
   const int64_t R = draft_ids.numel(), B = ctx_lens.numel();
+  KVS_CHECK_ARG(draft_ids.is_cuda() && draft_ids.scalar_type() == at::kInt, "commit_tree: int32 CUDA tensors");
+  if (out.empty()) {
+    // one piece of memory for all outputs
+    const torch::Tensor all = torch::empty({3 * B + R}, draft_ids.options());
+    out = {all.narrow(0, 0, B), all.narrow(0, B, R), all.narrow(0, B + R, B), all.narrow(0, 2 * B + R, B)};
+  }
+  KVS_CHECK_ARG(out.size() == 4, "commit_tree: four outputs");
+  const torch::Tensor &accepted = out[0], &path = out[1], &next_ids = out[2], &ctx_out = out[3];
   auto vec = [&](const torch::Tensor& t, int64_t n, const char* msg) {
     KVS_CHECK_ARG(t.is_cuda() && t.dim() == 1 && t.is_contiguous() && t.scalar_type() == at::kInt &&
                       t.numel() == n && t.device() == draft_ids.device(),
@@ -188,7 +205,8 @@ void commit_tree(torch::Tensor draft_ids, torch::Tensor target_ids, c10::optiona
     a.words = int(s.size(4) * item / 16);
     a.bs = int(c.size(3));
     a.num_slots = c.size(2) * c.size(3);
-    KVS_CHECK_ARG(int64_t(a.heads) * a.words * kMaxTree <= INT32_MAX, "commit_tree: K/V rows too long");
+    KVS_CHECK_ARG(int64_t(a.heads) * a.words * kMaxTree * s.size(0) * 2 <= INT32_MAX,
+                  "commit_tree: K/V rows too long");
     a.planes = int(s.size(0) * 2);
     a.planes_per_cta = int(std::max<int64_t>(1, std::min<int64_t>(a.planes, a.planes * B / kCommitCtas)));
   }
@@ -208,6 +226,7 @@ void commit_tree(torch::Tensor draft_ids, torch::Tensor target_ids, c10::optiona
   const int groups = (a.planes + a.planes_per_cta - 1) / a.planes_per_cta;
   tree_commit_kernel<<<dim3(unsigned(groups), unsigned(B)), kCommitThreads, 0, at::cuda::getCurrentCUDAStream()>>>(a);
   KVS_CUDA_CHECK(cudaGetLastError());
+  return out;
 }
 
 }  // namespace kvs

@@ -284,3 +284,26 @@ class LlamaShard:
         tok = dc.greedy(h, self.lm_head, self.vocab_begin, 2 * cfg.num_layers)
         dc.bump()
         return tok
+
+    def verify_step(self, ids: torch.Tensor, plan: "ops.StepPlan", tree_kv: torch.Tensor, kv_cache: torch.Tensor,
+                    block_tables: torch.Tensor, ctx_lens: torch.Tensor) -> torch.Tensor:
+        """Several drafted tokens per sequence (``plan``'s rows) against the
+        paged cache; their K and V go to ``tree_kv`` ``[L, 2, R, Hkv, D]``, not
+        into the cache.  Returns this shard's logits ``[R, vocab_local]``."""
+        cfg = self.cfg
+        R = ids.numel()
+        residual = ops.embedding(ids, self.embed)
+        h = ops.rmsnorm(residual, self.layers[0].in_norm, cfg.rms_eps)
+        for l, lw in enumerate(self.layers):
+            qkv = self._qkv(h, lw)
+            ops.rope_qkv(qkv, self.hq, self.hkv, self.D, plan.positions, self.cos_sin, tree_kv[l, 0], tree_kv[l, 1])
+            q = qkv[:, : self.hq * self.D].view(R, self.hq, self.D)
+            attn = ops.paged_tree_attention(q, tree_kv[l, 0], tree_kv[l, 1], kv_cache[l, 0], kv_cache[l, 1],
+                                            block_tables, ctx_lens, plan.indptr, tree_mask=plan.tree_mask,
+                                            scale=self.scale)
+            o = self._row_parallel(attn.view(R, self.hq * self.D), lw.o)
+            h = ops.rmsnorm(o, lw.post_norm, cfg.rms_eps, residual=residual)
+            d = self._mlp(h, lw)
+            nxt = self.layers[l + 1].in_norm if l + 1 < len(self.layers) else self.final_norm
+            h = ops.rmsnorm(d, nxt, cfg.rms_eps, residual=residual)
+        return ops.linear(h, self.lm_head)

@@ -24,6 +24,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
+from . import count_launches, device_status
 from ._ext import ext
 
 
@@ -46,11 +47,6 @@ class TreeCommit(NamedTuple):
     ctx_lens: torch.Tensor   # int32 [B] committed tokens after the step
 
 
-def _prelude():
-    from . import count_launches, device_status
-    return count_launches, device_status
-
-
 def plan_step(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torch.Tensor, held: torch.Tensor,
               free_queue: torch.Tensor, cursor: torch.Tensor, block_size: int, num_rows: int,
               parents: Optional[torch.Tensor] = None, max_tree: int = 64,
@@ -70,22 +66,14 @@ def plan_step(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torc
     depths; without it the rows are chains.  ``held`` and ``cursor`` may also
     be ``out.held`` and ``out.cursor`` (state updated in place).
     """
-    count_launches, device_status = _prelude()
-    dev = ctx_lens.device
-    if out is None:
-        def rows(*shape):
-            return torch.empty(shape, dtype=torch.int32, device=dev)
-        words = max(1, -(-int(max_tree) // 32))
-        out = StepPlan(rows(ctx_lens.numel() + 1), rows(num_rows), rows(num_rows), rows(num_rows),
-                       rows(num_rows, words) if parents is not None else None, torch.empty_like(held),
-                       torch.empty_like(cursor))
-    elif out.row_request.numel() != num_rows:
-        raise ValueError("plan_step: out was made for another number of rows")
-    count_launches(1)
-    ext().plan_step(ctx_lens, new_lens, block_tables, held, free_queue, cursor, int(block_size), parents, out.indptr,
-                    out.row_request, out.positions, out.slot_mapping, out.tree_mask, out.held, out.cursor,
-                    device_status(dev))
-    return out
+    # more than 1024 rows or requests: a second launch updates the state
+    count_launches(1 if max(num_rows, ctx_lens.numel()) <= 1024 else 2)
+    given = [] if out is None else [x for x in out if x is not None]
+    got = ext().plan_step(ctx_lens, new_lens, block_tables, held, free_queue, cursor, block_size, num_rows, parents,
+                          max_tree, given, device_status(ctx_lens.device))
+    if out is not None:
+        return out
+    return StepPlan(*got) if parents is not None else StepPlan(*got[:4], None, *got[4:])
 
 
 def paged_tree_attention(q: torch.Tensor, k_tree: torch.Tensor, v_tree: torch.Tensor, k_cache: torch.Tensor,
@@ -99,7 +87,6 @@ def paged_tree_attention(q: torch.Tensor, k_tree: torch.Tensor, v_tree: torch.Te
     to itself).  A row that sees nothing, and padding rows, give zeros.
     bf16 or fp16, head_dim 64 or 128, any number of query heads per KV head;
     ``k_tree`` / ``v_tree`` ``[R, Hkv, D]`` hold the step's own K and V."""
-    count_launches, device_status = _prelude()
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     if out is None:
@@ -144,7 +131,6 @@ def process_logits(logits: torch.Tensor, *, row_request: Optional[torch.Tensor] 
     ids outside it are ignored.  ``greedy`` int32 [R] receives the index of
     the largest value of ``out`` (lowest index of equal ones, the first NaN if
     there is one) and ``greedy_val`` fp32 [R] the value."""
-    count_launches, _ = _prelude()
     if out is None:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     count_launches(1 if greedy is None else 2)
@@ -165,12 +151,7 @@ def commit_tree(draft_ids: torch.Tensor, target_ids: torch.Tensor, parents: Opti
     ``[L, 2, blocks, block_size, Hkv, D]`` at ``slot_mapping[indptr[b] + k]``
     and their tokens written to ``tokens[b, ctx + k]`` (int32 [B, M]).  At
     most 1024 nodes a tree.  ``out.ctx_lens`` may be ``ctx_lens``."""
-    count_launches, device_status = _prelude()
-    dev = draft_ids.device
-    if out is None:
-        out = TreeCommit(torch.empty_like(ctx_lens), torch.empty_like(draft_ids), torch.empty_like(ctx_lens),
-                         torch.empty_like(ctx_lens))
     count_launches(1)
-    ext().commit_tree(draft_ids, target_ids, parents, indptr, ctx_lens, slot_mapping, tree_kv, kv_cache, tokens,
-                      out.accepted, out.path, out.next_ids, out.ctx_lens, device_status(dev))
-    return out
+    got = ext().commit_tree(draft_ids, target_ids, parents, indptr, ctx_lens, slot_mapping, tree_kv, kv_cache, tokens,
+                            [] if out is None else list(out), device_status(draft_ids.device))
+    return out if out is not None else TreeCommit(*got)

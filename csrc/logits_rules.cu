@@ -18,7 +18,10 @@
 // only the grammar bits, then the listed entries, where a drafted token's
 // count adds those on the row's own path.  With the rules inside the stream a
 // warp took their branches for nearly every piece, and with the block on one
-// row at a time it waited at barriers (8 trees of 32, V = 152064: 82 us).
+// row at a time it waited at barriers (8 trees of 32, V = 152064: 82 us; now
+// 68 us; 512 rows of 128256 fp32 with 8000 tokens each 200 us = 2.7 TB/s; one
+// row 7 us).  What bounds it now is instructions: every slice of a row reads
+// the whole history.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -486,7 +489,7 @@ void process_logits(torch::Tensor logits, torch::Tensor out, c10::optional<torch
     on(*tokens, at::kInt, "process_logits: tokens int32 [B, M]");
     KVS_CHECK_ARG(tokens->dim() == 2 && tokens->size(0) == B && tokens->stride(1) == 1 &&
                       tokens->size(1) + R < int64_t(kCountMask),
-                  "process_logits: tokens int32 [B, M] with contiguous rows, M below 2^20");
+                  "process_logits: tokens int32 [B, M] with contiguous rows, M + R below 2^19");
     a.tokens = tokens->data_ptr<int32_t>();
     a.tokens_stride = tokens->stride(0);
     a.tokens_len = int(tokens->size(1));

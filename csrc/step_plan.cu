@@ -14,7 +14,8 @@
 // The state may be updated in place, so its update comes after the last read
 // of the old one: a step of up to 1024 rows and requests is one CTA and one
 // launch, a larger one spreads its rows over the GPU and a second small kernel
-// follows (2048 requests, 60000 rows: 31 us as one cluster of 8 CTAs).
+// follows (2048 requests, 60000 rows: 10 us; 31 us as one cluster of 8 CTAs;
+// 8 trees of 16: 7.6 us).
 // Whole numbers and fixed order: the result does not depend on timing.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>

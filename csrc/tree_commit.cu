@@ -12,7 +12,8 @@
 // of one request and repeats the walk over its few hundred bytes in shared
 // memory, instead of waiting for another launch to write the path down; it
 // takes more planes as requests fill the GPU, so that the walk's latency is
-// paid once (128 requests, 56 planes: a CTA a plane 22.8 us).
+// paid once (128 trees, 56 planes of 1 KB rows: 20 us, 22.8 with a CTA a
+// plane; one tree of 32 layers 3.7 us).
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>

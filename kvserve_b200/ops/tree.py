@@ -63,7 +63,7 @@ def plan_step(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torc
     few blocks nobody gets one, rows without a block have slot -1, and the
     device status says so.  ``parents`` int32 [num_rows] (-1 for the root,
     index inside the tree otherwise) gives tree masks of ``max_tree`` bits and
-    depths; without it the rows are chains.  ``held`` and ``cursor`` may also
+    depths; without it the rows are chains.  At most 16384 requests.  ``held`` and ``cursor`` may also
     be ``out.held`` and ``out.cursor`` (state updated in place).
     """
     # more than 1024 rows or requests: a second launch updates the state
@@ -85,8 +85,10 @@ def paged_tree_attention(q: torch.Tensor, k_tree: torch.Tensor, v_tree: torch.Te
     D]``, any strides with contiguous head rows) and the tree rows of its
     request whose bit is set in ``tree_mask[r]`` (without a mask: the rows up
     to itself).  A row that sees nothing, and padding rows, give zeros.
-    bf16 or fp16, head_dim 64 or 128, any number of query heads per KV head;
-    ``k_tree`` / ``v_tree`` ``[R, Hkv, D]`` hold the step's own K and V."""
+    bf16 or fp16, head_dim 64 or 128, up to 128 query heads per KV head, a
+    positive ``scale``; head rows start at 16-byte boundaries.  ``k_tree`` /
+    ``v_tree`` ``[R, Hkv, D]`` hold the step's own K and V.  Probabilities are
+    rounded to the K/V type before the product with V; sums are fp32."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     if out is None:
@@ -125,7 +127,8 @@ def process_logits(logits: torch.Tensor, *, row_request: Optional[torch.Tensor] 
     their position is at least ``prompt_lens[b]``.  ``row_request`` [R] maps
     rows to requests (-1: no rules but the grammar; None: row r is request r).
     ``bias_ids`` / ``bias_values`` [B, K]: ids below 0 are padding, an id
-    listed twice gets the sum.  ``allowed`` int32 [A, ceil(V / 32)] holds bit
+    listed twice gets the sum; at most 2047 a request.  ``tokens`` may be up to
+    2^19 wide (less the number of rows).  ``allowed`` int32 [A, ceil(V / 32)] holds bit
     masks over the columns, ``allowed_index`` [R] names each row's mask (-1:
     none).  With ``vocab_begin`` the columns are a shard of the vocabulary;
     ids outside it are ignored.  ``greedy`` int32 [R] receives the index of

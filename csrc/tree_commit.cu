@@ -52,6 +52,8 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const Commi
   const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int lo = min(max(a.indptr[b], 0), a.R), hi = min(max(a.indptr[b + 1], lo), a.R);
   const int n = min(hi - lo, kMaxTree);
+  // Before the barriers: `ctx_out` may be `ctx`, and its store comes after them.
+  const int ctx = blockIdx.x == 0 ? a.ctx[b] : 0;
   for (int i = tid; i < n; i += kCommitThreads) {
     s_draft[i] = a.drafts[lo + i];
     s_target[i] = a.targets[lo + i];
@@ -79,7 +81,6 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const Commi
   __syncthreads();
   const int len = s_len;
   if (blockIdx.x == 0) {
-    const int ctx = a.ctx[b];
     for (int k = tid; k < hi - lo; k += kCommitThreads) {
       a.path[lo + k] = k < len ? int(s_path[k]) : -1;
       if (k < len && a.tokens != nullptr) {

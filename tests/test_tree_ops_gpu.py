@@ -544,6 +544,38 @@ def test_commit_tree(new, L, hkv, D, bs, dtype, chain):
     assert max(len(p) for p in paths) > (1 if sum(new) > 4 else 0)
 
 
+def test_commit_tree_updates_context_lengths_in_place():
+    """Accepted chains longer than a block of threads, with ``ctx_lens`` as the
+    output too: tokens and lengths are those of separate outputs."""
+    ops = _ops()
+    new = [300, 1, 700, 64, 1024, 33] * 4
+    R, B = sum(new), len(new)
+    indptr = np.concatenate([[0], np.cumsum(new)]).tolist()
+    drafts = [1 + r for r in range(R)]
+    targets = drafts[1:] + [0]  # every node carries what was chosen after the one before: all accepted
+    ctx = _i32([(37 * b) % 50 for b in range(B)])
+    width = 50 + max(new)
+
+    def commit(out, ctx):
+        tokens = torch.full((B, width), -5, dtype=torch.int32, device="cuda")
+        c = ops.commit_tree(_i32(drafts), _i32(targets), None, _i32(indptr), ctx, _i32([0] * R), tokens=tokens, out=out)
+        ops.check_device_status()
+        return c, tokens
+    want, want_tokens = commit(None, ctx)
+    assert want.accepted.tolist() == new and want.ctx_lens.tolist() == (ctx + _i32(new)).tolist()
+    for b, n in enumerate(new):
+        c = ctx[b].item()
+        assert want_tokens[b, c:c + n].tolist() == drafts[indptr[b]:indptr[b + 1]]
+        assert (want_tokens[b, :c] == -5).all() and (want_tokens[b, c + n:] == -5).all()
+    for _ in range(20):
+        state = ctx.clone()
+        out = ops.TreeCommit(torch.empty_like(ctx), torch.empty(R, dtype=torch.int32, device="cuda"),
+                             torch.empty_like(ctx), state)
+        got, tokens = commit(out, state)
+        assert got.ctx_lens is state and torch.equal(tokens, want_tokens)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_commit_tree_lowest_child_wins_and_strided_rows():
     """Two children carry the accepted token; K/V rows and cache are views."""
     ops = _ops()

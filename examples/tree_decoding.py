@@ -25,14 +25,15 @@ def main() -> None:
     ap.add_argument("--repetition", type=float, default=1.0)
     args = ap.parse_args()
     cfg = get_config(args.model)
-    model = LlamaShard(cfg, device="cuda:0", max_position=4096)
+    max_len = args.prompt + args.new_tokens + 64
+    model = LlamaShard(cfg, device="cuda:0", max_position=max_len)
     g = torch.Generator().manual_seed(0)
     prompts = [torch.randint(0, cfg.vocab, (args.prompt // 4 + 1,), generator=g).repeat(4)[:args.prompt].to(torch.int32)
                for _ in range(args.requests)]
     rules = {"repetition": torch.full((args.requests,), args.repetition, device="cuda:0")}
     blocks = args.requests * ((args.prompt + args.new_tokens) // 16 + 4)
     for name, nodes in (("one token a step", 1), ("trees of 16", 16)):
-        dec = TreeDecoder(model, num_blocks=blocks, max_len=args.prompt + args.new_tokens + 64, max_tree=nodes)
+        dec = TreeDecoder(model, num_blocks=blocks, max_len=max_len, max_tree=nodes)
         dec.generate(prompts, 2, rules)  # warm-up
         torch.cuda.synchronize()
         t = time.perf_counter()

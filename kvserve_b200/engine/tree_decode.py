@@ -72,6 +72,8 @@ class TreeDecoder:
             raise ValueError("tree decoding runs on one GPU (TP size 1)")
         if not 1 <= max_tree <= 64:
             raise ValueError("max_tree must be 1 to 64")
+        if max_len > model.cos_sin.shape[0]:
+            raise ValueError(f"max_len {max_len} exceeds the model's rotary table (max_position {model.cos_sin.shape[0]})")
         self.model, self.max_len, self.max_tree, self.propose = model, max_len, max_tree, propose
         cfg, dev = model.cfg, model.device
         self.block_size = block_size

@@ -126,3 +126,14 @@ def test_refusals():
         TreeDecoder(SimpleNamespace(tp_size=2), 4, 64)
     with pytest.raises(ValueError, match="max_tree"):
         TreeDecoder(SimpleNamespace(tp_size=1), 4, 64, max_tree=65)
+
+
+def test_max_len_beyond_the_rotary_table_is_refused():
+    """Refused on the host: the rotary kernels read the table by position."""
+    from types import SimpleNamespace
+    from kvserve_b200.engine.tree_decode import TreeDecoder
+    cfg = SimpleNamespace(num_layers=1)
+    model = SimpleNamespace(tp_size=1, cfg=cfg, device=torch.device("cpu"), hkv=1, D=64, cos_sin=torch.zeros(100, 64))
+    with pytest.raises(ValueError, match="rotary table"):
+        TreeDecoder(model, 4, 101)
+    assert TreeDecoder(model, 4, 100).max_len == 100

@@ -7,13 +7,17 @@ drafter (looking the last tokens up earlier in the text) finds continuations.
 Prints the tokens per verify step with and without drafts.
 """
 import argparse
+import os
+import sys
 import time
 
 import torch
 
-from kvserve_b200.engine.tree_decode import TreeDecoder
-from kvserve_b200.models.config import get_config
-from kvserve_b200.models.llama import LlamaShard
+sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))  # run in a source tree
+
+from kvserve_b200.engine.tree_decode import TreeDecoder  # noqa: E402
+from kvserve_b200.models.config import get_config  # noqa: E402
+from kvserve_b200.models.llama import LlamaShard  # noqa: E402
 
 
 def main() -> None:

@@ -137,3 +137,15 @@ def test_max_len_beyond_the_rotary_table_is_refused():
     with pytest.raises(ValueError, match="rotary table"):
         TreeDecoder(model, 4, 101)
     assert TreeDecoder(model, 4, 100).max_len == 100
+
+
+def test_the_example_starts_from_the_source_tree(tmp_path):
+    """Its documented command finds the package without an installation."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    env = {k: v for k, v in os.environ.items() if k != "PYTHONPATH"}
+    run = subprocess.run([sys.executable, os.path.join(root, "examples", "tree_decoding.py"), "--help"], cwd=tmp_path,
+                         env=env, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "--new-tokens" in run.stdout, run.stderr

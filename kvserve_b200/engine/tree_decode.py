@@ -65,6 +65,13 @@ class TreeResult:
     steps: int            # verify steps that the request took part in
 
 
+@dataclass
+class _Requests:
+    ctx: torch.Tensor     # int32 [B] committed tokens
+    held: torch.Tensor    # int32 [B] blocks held
+    tables: torch.Tensor  # int32 [B, W]
+
+
 class TreeDecoder:
     def __init__(self, model: LlamaShard, num_blocks: int, max_len: int, block_size: int = 16, max_tree: int = 16,
                  propose: Callable[[Sequence[int], int], Drafts] = lookup_drafts):
@@ -106,28 +113,35 @@ class TreeDecoder:
         tokens = torch.zeros(B, self.max_len, dtype=torch.int32, device=dev)
         for b, h in enumerate(history):
             tokens[b, :lens[b]] = self._ints(h)
-        held = torch.zeros(B, dtype=torch.int32, device=dev)
+        none = torch.zeros(B, dtype=torch.int32, device=dev)
+        req = _Requests(none, none, tables)
         # the prompt without its last token, which is the root of the first tree
         new = self._ints(n - 1 for n in lens)
-        ctx = torch.zeros(B, dtype=torch.int32, device=dev)
-        plan = ops.plan_step(ctx, new, tables, held, self.free_queue, self.cursor, bs, sum(lens) - B)
-        held, self.cursor = plan.held, plan.cursor
         try:
-            ops.check_device_status(dev)
+            plan = self._plan(req, new, sum(lens) - B)
             self._prefill(history, plan)
-            ctx = new
+            req.ctx = new
             prompt_lens = self._ints(lens)
             results = [TreeResult([], 0) for _ in range(B)]
             live = list(range(B))
             while live:
-                ctx, held = self._step(history, results, live, ctx, held, tables, tokens, prompt_lens, rules or {},
-                                       max_new_tokens, stop)
+                self._step(history, results, live, req, tokens, prompt_lens, rules or {}, max_new_tokens, stop)
                 live = [b for b in live if len(results[b].tokens) < max_new_tokens
                         and not (results[b].tokens and results[b].tokens[-1] == stop)]
             return results
         finally:  # all blocks go back
-            end = ops.plan_step(ctx, torch.full_like(ctx, -1), tables, held, self.free_queue, self.cursor, bs, 0)
-            self.cursor = end.cursor
+            self.cursor = ops.plan_step(req.ctx, torch.full_like(none, -1), tables, req.held, self.free_queue,
+                                        self.cursor, bs, 0).cursor
+
+    def _plan(self, req: _Requests, new: torch.Tensor, rows: int, parents=None) -> "ops.StepPlan":
+        """Plan of a step.  The held blocks and the ring's cursor advance with
+        it at once, so that whatever fails afterwards, what the plan took is
+        known and goes back."""
+        plan = ops.plan_step(req.ctx, new, req.tables, req.held, self.free_queue, self.cursor, self.block_size, rows,
+                             parents=parents, max_tree=self.max_tree)
+        req.held, self.cursor = plan.held, plan.cursor
+        ops.check_device_status(self.model.device)  # blocks ran out, or a broken tree
+        return plan
 
     def _prefill(self, history: list, plan: "ops.StepPlan") -> None:
         m, at = self.model, 0
@@ -144,9 +158,9 @@ class TreeDecoder:
             self.kv[:, 1].view(L, nb * bs, hkv, D)[:, slots] = v
             at += n
 
-    def _step(self, history, results, live, ctx, held, tables, tokens, prompt_lens, rules, max_new, stop):
-        m, bs = self.model, self.block_size
-        B = ctx.numel()
+    def _step(self, history, results, live, req: _Requests, tokens, prompt_lens, rules, max_new, stop):
+        m = self.model
+        B = len(history)
         new, drafts, parents = [0] * B, [], []
         for b in live:
             room = min(self.max_tree, max_new - len(results[b].tokens))
@@ -158,19 +172,17 @@ class TreeDecoder:
         ids = self._ints(drafts)
         par = self._ints(parents)
         R = len(drafts)
-        plan = ops.plan_step(ctx, self._ints(new), tables, held, self.free_queue, self.cursor, bs, R, parents=par,
-                             max_tree=self.max_tree)
-        self.cursor = plan.cursor
-        ops.check_device_status(m.device)  # blocks ran out: nothing has been written
+        plan = self._plan(req, self._ints(new), R, parents=par)
         L, _, _, _, hkv, D = self.kv.shape
         tree_kv = torch.empty(L, 2, R, hkv, D, dtype=self.kv.dtype, device=self.kv.device)
-        logits = m.verify_step(ids, plan, tree_kv, self.kv, tables, ctx)
+        logits = m.verify_step(ids, plan, tree_kv, self.kv, req.tables, req.ctx)
         chosen = torch.empty(R, dtype=torch.int32, device=m.device)
-        ops.process_logits(logits, row_request=plan.row_request, tokens=tokens, token_lens=ctx, prompt_lens=prompt_lens,
+        ops.process_logits(logits, row_request=plan.row_request, tokens=tokens, token_lens=req.ctx, prompt_lens=prompt_lens,
                            draft_ids=ids, indptr=plan.indptr, tree_mask=plan.tree_mask, positions=plan.positions,
                            out=logits, greedy=chosen, **rules)
-        done = ops.commit_tree(ids, chosen, par, plan.indptr, ctx, plan.slot_mapping, tree_kv=tree_kv,
+        done = ops.commit_tree(ids, chosen, par, plan.indptr, req.ctx, plan.slot_mapping, tree_kv=tree_kv,
                                kv_cache=self.kv, tokens=tokens)
+        req.ctx = done.ctx_lens
         # the drafts of the next step come from the host: one read back a step
         path, accepted, chosen = done.path.tolist(), done.accepted.tolist(), chosen.tolist()
         row = 0
@@ -182,4 +194,3 @@ class TreeDecoder:
             results[b].tokens += got
             results[b].steps += 1
             row += new[b]
-        return done.ctx_lens, plan.held

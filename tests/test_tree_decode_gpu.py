@@ -149,3 +149,24 @@ def test_the_example_starts_from_the_source_tree(tmp_path):
     run = subprocess.run([sys.executable, os.path.join(root, "examples", "tree_decoding.py"), "--help"], cwd=tmp_path,
                          env=env, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and "--new-tokens" in run.stdout, run.stderr
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fault", ["rule", "parent"])
+def test_a_step_that_fails_after_its_plan_gives_its_blocks_back(fault):
+    """The step's plan takes a block (the prompt ends a block) before the rules
+    are refused, or before the broken tree is reported."""
+    from kvserve_b200.engine.tree_decode import TreeDecoder
+    model = _model()
+    prompt = torch.arange(33, dtype=torch.int32)  # 32 committed tokens: two whole blocks of 16
+
+    def broken(history, nodes):  # a parent that comes later
+        return [5, 6], [2, 0]
+    dec = TreeDecoder(model, num_blocks=16, max_len=128, propose=broken if fault == "parent" else lambda h, n: ([], []))
+    rules = {"repetition": torch.full((1,), 1.1)} if fault == "rule" else {}  # not on the GPU
+    for _ in range(3):
+        with pytest.raises((ValueError, RuntimeError)):
+            dec.generate([prompt], 8, rules=rules)
+        assert dec.free_blocks() == 16
+    dec.propose = lambda h, n: ([], [])
+    assert len(dec.generate([prompt], 8)[0].tokens) == 8 and dec.free_blocks() == 16

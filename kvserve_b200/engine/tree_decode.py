@@ -109,6 +109,11 @@ class TreeDecoder:
             return []
         if min(lens) < 1 or max(lens) + max_new_tokens + self.max_tree > self.max_len:
             raise ValueError("prompt is empty, or prompt and new tokens exceed max_len")
+        if max_new_tokens < 0:
+            raise ValueError("max_new_tokens is negative")
+        results = [TreeResult([], 0) for _ in range(B)]
+        if max_new_tokens == 0:
+            return results
         tables = torch.zeros(B, -(-self.max_len // bs), dtype=torch.int32, device=dev)
         tokens = torch.zeros(B, self.max_len, dtype=torch.int32, device=dev)
         for b, h in enumerate(history):
@@ -122,7 +127,6 @@ class TreeDecoder:
             self._prefill(history, plan)
             req.ctx = new
             prompt_lens = self._ints(lens)
-            results = [TreeResult([], 0) for _ in range(B)]
             live = list(range(B))
             while live:
                 self._step(history, results, live, req, tokens, prompt_lens, rules or {}, max_new_tokens, stop)

@@ -170,3 +170,13 @@ def test_a_step_that_fails_after_its_plan_gives_its_blocks_back(fault):
         assert dec.free_blocks() == 16
     dec.propose = lambda h, n: ([], [])
     assert len(dec.generate([prompt], 8)[0].tokens) == 8 and dec.free_blocks() == 16
+
+
+@pytest.mark.gpu
+def test_no_new_tokens():
+    from kvserve_b200.engine.tree_decode import TreeDecoder
+    dec = TreeDecoder(_model(), num_blocks=16, max_len=128)
+    out = dec.generate([torch.arange(n, dtype=torch.int32) for n in (1, 20)], 0)
+    assert [(r.tokens, r.steps) for r in out] == [([], 0), ([], 0)] and dec.free_blocks() == 16
+    with pytest.raises(ValueError, match="max_new_tokens"):
+        dec.generate([torch.arange(20, dtype=torch.int32)], -1)

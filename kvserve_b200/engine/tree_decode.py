@@ -107,7 +107,7 @@ class TreeDecoder:
         lens = [len(h) for h in history]
         if B == 0:
             return []
-        if min(lens) < 1 or max(lens) + max_new_tokens + self.max_tree > self.max_len:
+        if min(lens) < 1 or max(lens) + max_new_tokens > self.max_len:
             raise ValueError("prompt is empty, or prompt and new tokens exceed max_len")
         if max_new_tokens < 0:
             raise ValueError("max_new_tokens is negative")

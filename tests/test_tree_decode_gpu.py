@@ -180,3 +180,18 @@ def test_no_new_tokens():
     assert [(r.tokens, r.steps) for r in out] == [([], 0), ([], 0)] and dec.free_blocks() == 16
     with pytest.raises(ValueError, match="max_new_tokens"):
         dec.generate([torch.arange(20, dtype=torch.int32)], -1)
+
+
+@pytest.mark.gpu
+def test_text_may_fill_max_len():
+    """Prompt and new tokens of exactly max_len give the tokens of a decoder
+    with room to spare; one more is refused."""
+    from kvserve_b200.engine.tree_decode import TreeDecoder
+    model = _model()
+    prompt = torch.arange(7, dtype=torch.int32).repeat(6)[:40]
+    roomy = TreeDecoder(model, num_blocks=16, max_len=128).generate([prompt], 9)[0]
+    dec = TreeDecoder(model, num_blocks=16, max_len=49)
+    tight = dec.generate([prompt], 9)[0]
+    assert tight.tokens == roomy.tokens and tight.steps == roomy.steps and len(tight.tokens) == 9
+    with pytest.raises(ValueError, match="max_len"):
+        dec.generate([prompt], 10)

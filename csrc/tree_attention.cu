@@ -39,6 +39,13 @@ constexpr int BM = 128;      // query rows of a tile (the MMA's M)
 constexpr int BN = 64;       // tokens of a K/V tile
 constexpr int kThreads = 448;  // warps 0..3 and 4..7 softmax of the two streams, 8 and 9 loaders, 10..13 MMA issuers
 constexpr float kRescaleThreshold = 8.0f;  // log2: P stays below 2^8 between rescalings
+// log2 of a factor on P, its row sums and O that cancels in the end.  fp16 has
+// normal numbers down to 2^-14 only: with 2^7, probabilities keep all their
+// bits down to 2^-21 of the largest one and end at 2^-32 (without it 2^-14 and
+// 2^-25: many tokens under one of large weight lost their share); 2^(8 + 7) is
+// below fp16's largest number.  bf16 has the exponents of fp32.
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 7.0f : 0.0f;
 
 struct TreeArgs {
   const void *q, *kt, *vt, *kc, *vc;
@@ -757,7 +764,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // rescale lazily: only when the maximum grew by more than the threshold
           const bool rescale = mxs > m_ref + kRescaleThreshold;
           const float m_use = rescale ? mxs : m_ref;
-          const float neg_m = m_use == -INFINITY ? 0.f : -m_use;  // nothing visible yet: all P are 0
+          const float neg_m = m_use == -INFINITY ? 0.f : kLift<T> - m_use;  // nothing visible yet: all P are 0
           float sa[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
           __syncwarp();
 #pragma unroll

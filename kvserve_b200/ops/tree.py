@@ -88,7 +88,8 @@ def paged_tree_attention(q: torch.Tensor, k_tree: torch.Tensor, v_tree: torch.Te
     bf16 or fp16, head_dim 64 or 128, up to 128 query heads per KV head, a
     positive ``scale``; head rows start at 16-byte boundaries.  ``k_tree`` /
     ``v_tree`` ``[R, Hkv, D]`` hold the step's own K and V.  Probabilities are
-    rounded to the K/V type before the product with V; sums are fp32."""
+    rounded to the K/V type before the product with V (fp16: with all bits
+    down to 2^-21 of the row's largest one, none below 2^-32); sums are fp32."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     if out is None:

@@ -172,6 +172,27 @@ def test_tree_attention_scale_and_sharp_scores():
     _check_attention(x, [5, 5], [300, 90], sets, _mask_tensor(sets, 1), scale=0.11)
 
 
+@pytest.mark.parametrize("drop", [9, 19.5, 25.2])
+def test_tree_attention_fp16_tail_under_a_sink(drop):
+    """Each request's fourth token takes nearly all of the weight and has a
+    zero V; the result is what the many others (2^-drop of its weight each)
+    leave.  Enough requests that a share holds many tiles with the sink's
+    maximum: the others' probabilities must not lose bits to the smallest
+    numbers that fp16 has."""
+    new, ctx, D = [2] * 96, [1000 + b for b in range(96)], 128
+    x = _attention_inputs(new, ctx, 8, 2, D, 16, torch.float16, poison=False)
+    x["q"][:] = 1.0
+    x["kc"] *= 2.0 ** -7                          # scores of the others: within a few hundredths of 0
+    x["kt"] *= 2.0 ** -7
+    x["vc"] = x["vc"].abs() + 0.5                 # nothing cancels
+    x["vt"] = x["vt"].abs() + 0.5
+    first = x["table"][:, 0].long()
+    x["kc"][first, 3] = drop * math.log(2.0) / D ** 0.5  # a score of drop * ln 2
+    x["vc"][first, 3] = 0.0
+    sets = [s for n in new for s in _paths([-1] + [0] * (n - 1))]
+    _check_attention(x, new, ctx, sets, _mask_tensor(sets, 1))
+
+
 def test_tree_attention_rows_that_see_nothing_are_zero():
     new, ctx = [4, 3], [0, 50]
     x = _attention_inputs(new, ctx, 8, 2, 128, 16, torch.bfloat16)

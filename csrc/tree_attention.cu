@@ -324,7 +324,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   // is asked for instead of padded for, and checked
   extern __shared__ __align__(1024) uint8_t smem[];
   if (smem_u32(smem) & 1023) {
-    if (threadIdx.x == 0) atomicCAS(a.err, 0u, uint32_t(kStatusBadSize));
+    if (threadIdx.x == 0) {
+      a.meta[blockIdx.x] = make_int4(0, 0, 1, 0);  // no tiles: the joining kernel reads it all the same
+      atomicCAS(a.err, 0u, uint32_t(kStatusBadSize));
+    }
     return;
   }
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Lay::OFF_BAR);

@@ -158,6 +158,16 @@ def test_tree_attention_random_trees(new, ctx, hq, hkv, D, bs, dtype, layout):
     _check_attention(x, new, ctx, sets, _mask_tensor(sets, words))
 
 
+@pytest.mark.parametrize("group,D", [(17, 128), (20, 64), (24, 128), (64, 128), (128, 64)])
+def test_tree_attention_large_groups(group, D):
+    """More than 16 query heads a KV head, numbers among them that do not
+    divide a row tile."""
+    new, ctx = [9, 1, 15], [130, 0, 77]
+    x = _attention_inputs(new, ctx, 2 * group, 2, D, 16, torch.bfloat16)
+    sets = [s for n in new for s in _paths(_random_tree(random.Random(group), n))]
+    _check_attention(x, new, ctx, sets, _mask_tensor(sets, 1))
+
+
 @pytest.mark.parametrize("new,ctx", [([1, 1, 1], [0, 64, 200]), ([200], [100]), ([70, 3], [0, 33])])
 def test_tree_attention_without_a_mask_is_causal(new, ctx):
     x = _attention_inputs(new, ctx, 8, 2, 128, 16, torch.bfloat16)
@@ -463,6 +473,36 @@ def test_plan_step_updates_its_state_in_place():
         assert sorted(owned + free) == list(range(pool))
         slots = plan.slot_mapping[: plan.indptr[-1]].tolist()
         assert len(set(slots)) == len(slots) and min(slots, default=0) >= 0
+
+
+def test_plan_step_over_several_blocks_updates_its_state_in_place():
+    """As above with more rows than one block of threads plans (the state is
+    then written by a second launch), against separate outputs."""
+    ops = _ops()
+    rng = random.Random(8)
+    B, bs, pool, W = 70, 16, 3000, 60
+    R = B * 33
+    ctx = _i32([0] * B)
+    table, queue = torch.zeros(B, W, dtype=torch.int32, device="cuda"), _i32(list(range(pool)))
+    held, cursor = _i32([0] * B), torch.tensor([0, pool], device="cuda")
+    state = None
+    for _ in range(25):
+        new = _i32([rng.choice([-1, 0, 3, 33, 33]) for _ in range(B)])
+        t2, q2 = table.clone(), queue.clone()
+        want = ops.plan_step(ctx, new, t2, held, q2, cursor, bs, R)
+        if state is None:
+            state = want._replace(held=held.clone(), cursor=cursor.clone())
+        got = ops.plan_step(ctx, new, table, state.held, queue, state.cursor, bs, R, out=state)
+        ops.check_device_status()
+        assert got is state and torch.equal(table, t2) and torch.equal(queue, q2)
+        for a, b in zip(got, want):
+            assert a is None and b is None or torch.equal(a, b)
+        held, cursor = state.held.clone(), state.cursor.clone()
+        ctx = torch.where(new < 0, torch.zeros_like(ctx), ctx + new.clamp(min=0))
+        ctx = ctx.clamp(max=(W - 3) * bs)
+        held_list, (head, tail) = held.tolist(), cursor.tolist()
+        owned = [v for b in range(B) for v in table[b, :held_list[b]].tolist()]
+        assert sorted(owned + [queue[i % pool].item() for i in range(head, tail)]) == list(range(pool))
 
 
 def test_plan_step_reports_what_does_not_fit():

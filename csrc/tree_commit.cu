@@ -26,7 +26,7 @@ namespace {
 
 constexpr int kCommitThreads = 256;
 constexpr int kMaxTree = 1024;
-constexpr int kCommitCtas = 8 * kNumSMs;  // 2048 threads an SM
+constexpr int kCommitCtas = 8 * kNumSMs;  // CTAs of a full GPU's batch; 40 registers a thread let six on an SM at a time
 
 struct CommitArgs {
   const int32_t *drafts, *targets, *parents, *indptr, *ctx, *slots;
@@ -48,12 +48,12 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const Commi
   pdl_trigger();
   __shared__ int s_draft[kMaxTree], s_target[kMaxTree], s_parent[kMaxTree], s_slot[kMaxTree];
   __shared__ uint16_t s_path[kMaxTree];
-  __shared__ int s_len;
+  __shared__ int s_len, s_ctx;
   const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int lo = min(max(a.indptr[b], 0), a.R), hi = min(max(a.indptr[b + 1], lo), a.R);
   const int n = min(hi - lo, kMaxTree);
-  // Before the barriers: `ctx_out` may be `ctx`, and its store comes after them.
-  const int ctx = blockIdx.x == 0 ? a.ctx[b] : 0;
+  // read before the barriers: `ctx_out` may be `ctx`, and its store comes after them
+  if (tid == 0) s_ctx = a.ctx[b];
   for (int i = tid; i < n; i += kCommitThreads) {
     s_draft[i] = a.drafts[lo + i];
     s_target[i] = a.targets[lo + i];
@@ -81,6 +81,7 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const Commi
   __syncthreads();
   const int len = s_len;
   if (blockIdx.x == 0) {
+    const int ctx = s_ctx;
     for (int k = tid; k < hi - lo; k += kCommitThreads) {
       a.path[lo + k] = k < len ? int(s_path[k]) : -1;
       if (k < len && a.tokens != nullptr) {

@@ -132,6 +132,7 @@ class TreeDecoder:
                 self._step(history, results, live, req, tokens, prompt_lens, rules or {}, max_new_tokens, stop)
                 live = [b for b in live if len(results[b].tokens) < max_new_tokens
                         and not (results[b].tokens and results[b].tokens[-1] == stop)]
+            ops.check_device_status(dev)  # the last step's; the others' were read after the next plan
             return results
         finally:  # all blocks go back
             self.cursor = ops.plan_step(req.ctx, torch.full_like(none, -1), tables, req.held, self.free_queue,

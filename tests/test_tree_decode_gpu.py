@@ -195,3 +195,23 @@ def test_text_may_fill_max_len():
     assert tight.tokens == roomy.tokens and tight.steps == roomy.steps and len(tight.tokens) == 9
     with pytest.raises(ValueError, match="max_len"):
         dec.generate([prompt], 10)
+
+
+@pytest.mark.gpu
+def test_an_error_in_the_last_step_is_raised(monkeypatch):
+    """What the kernels of the last step report does not wait for a later call."""
+    from kvserve_b200 import ops
+    from kvserve_b200.engine.tree_decode import TreeDecoder
+    model = _model()
+    dec = TreeDecoder(model, num_blocks=16, max_len=128)
+    verify = model.verify_step
+
+    def failing(*args):
+        logits = verify(*args)
+        ops.device_status(model.device)[0] = 1  # as a kernel whose wait ran out does
+        return logits
+    monkeypatch.setattr(model, "verify_step", failing)
+    with pytest.raises(RuntimeError, match="timeout"):
+        dec.generate([torch.arange(20, dtype=torch.int32)], 1)
+    assert dec.free_blocks() == 16
+    ops.check_device_status(model.device)

@@ -17,11 +17,15 @@
 // item leaves an fp32 record (row maximum, row sum, O) that a second small
 // kernel joins in a fixed order.
 //
-// Measured (B200, device time, 128-wide heads): 64 requests of 16 nodes over
-// up to 2900 tokens, 32/8 heads, 130 us = 4.3 TB/s (HBM floor 87 us); 128
-// single tokens over 2047, 28/4 heads, 88 us = 4.3 TB/s; one tree of 64 over
-// 131000 tokens, 64/8 heads, 321 us = 855 TFLOP/s (tensor floor 163 us); one
-// tree of 8 over 700 tokens 16.6 us, all latency.
+// Measured (B200, device time in a CUDA graph; called one after another in
+// brackets; 128-wide heads): 64 requests of 16 nodes over up to 2900 tokens,
+// 32/8 heads, 131 to 134 us = 4.2 to 4.3 TB/s (142; HBM floor 87); 128 single
+// tokens over 2047, 28/4 heads, fp16, 87 us = 4.4 TB/s (90; floor 59); one
+// tree of 64 over 131000 tokens, 64/8 heads, 324 us = 848 TFLOP/s (331; tensor
+// floor 163); one tree of 8 over 700 tokens 16.2 us (18.2), all latency.  The
+// 64 requests with 64-wide heads 113 us (floor 44), with blocks of 8 tokens,
+// whose TMA boxes are half as large, 156 us.  Blocks that are no multiple of 8
+// tokens go through one copying warp each for K and V: 2404 us.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -276,7 +280,8 @@ struct Layout {
 static_assert(Layout<128>::SMEM <= 232448 && Layout<64>::SMEM <= 232448, "shared memory of one SM");
 
 // Copies the rows of one K or V tile with plain loads (one warp): caches
-// whose blocks TMA boxes do not tile.  Rows at or past `valid` become zero.
+// whose blocks TMA boxes do not tile (64 requests over 2900 tokens 2404 us
+// instead of 134).  Rows at or past `valid` become zero.
 template <int D>
 __device__ __forceinline__ void copy_tile(uint8_t* dst, const uint16_t* src, int64_t row_stride, int valid, int lane) {
   constexpr int C = D / 8;
@@ -932,7 +937,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // a round: their maxima and sums first (one lane a record and row), then O,
 // with the loads of four records in flight.  Rows of no request become zero.
 // All of it is a few dependent reads from L2: bound by latency (64 requests:
-// the call takes 130 us; 142 with a block on a batch of rows at a time).
+// the call took 130 us in a CUDA graph; 142 with a block on a batch of rows at
+// a time).
 constexpr int kMergeThreads = 256;
 constexpr int kMergeSplit = 4;  // CTAs a worker
 

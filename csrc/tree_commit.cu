@@ -7,13 +7,15 @@
 // token.  The K/V rows of the path go from the step's staging rows to the
 // cache slots of positions ctx, ctx + 1, ..., for every layer in one launch.
 //
-// Each row of K or V is read and written once: bound by HBM for a full batch
-// and by latency for a single request.  A CTA takes some (layer, part) planes
+// Each row of K or V is read and written once; a single request is bound by
+// latency.  A full batch is not bound by HBM (11 % of it) but by the walk, at
+// whose barriers most stalled warps wait, and the index arithmetic of every
+// 16-byte word (55 % of the issue slots).  A CTA takes some (layer, part) planes
 // of one request and repeats the walk over its few hundred bytes in shared
 // memory, instead of waiting for another launch to write the path down; it
 // takes more planes as requests fill the GPU, so that the walk's latency is
 // paid once (128 trees, 56 planes of 1 KB rows: 20 us, 22.8 with a CTA a
-// plane; one tree of 32 layers 3.7 us).
+// plane; one tree of 32 layers 3.7 us; in a CUDA graph).
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>

@@ -4,15 +4,17 @@ Every step verifies a small tree of drafted tokens per request in one pass of
 the model: :func:`kvserve_b200.ops.plan_step` lays the rows out and hands out
 KV blocks on the GPU, :meth:`LlamaShard.verify_step` runs the model with
 :func:`~kvserve_b200.ops.paged_tree_attention`,
-:func:`~kvserve_b200.ops.process_logits` applies penalties, biases and grammar
-masks and picks the model's choice after every node, and
+:func:`~kvserve_b200.ops.process_logits` applies penalties and biases and picks
+the model's choice after every node, and
 :func:`~kvserve_b200.ops.commit_tree` accepts a path and moves its K/V rows
 into the paged cache.  A step yields one to ``max_tree`` tokens a request; the
 result is that of one-token greedy decoding under the same rules (up to the
-rounding of differently shaped products).
+rounding of differently shaped products).  Steps are launched kernel by kernel,
+not from a CUDA graph.  Grammar masks belong to rows, not to requests: whoever
+needs them calls the operators one by one.
 
     dec = TreeDecoder(model, num_blocks=4096, max_len=4096)
-    out = dec.generate(prompts, 128, rules={"repetition": torch.full((B,), 1.1)})
+    out = dec.generate(prompts, 128, rules={"repetition": torch.full((B,), 1.1, device="cuda")})
 
 ``propose(history, max_nodes) -> (tokens, parents)`` drafts for one request;
 the default looks the last tokens up earlier in the request's own text.
@@ -80,7 +82,8 @@ class TreeDecoder:
         if not 1 <= max_tree <= 64:
             raise ValueError("max_tree must be 1 to 64")
         if max_len > model.cos_sin.shape[0]:
-            raise ValueError(f"max_len {max_len} exceeds the model's rotary table (max_position {model.cos_sin.shape[0]})")
+            raise ValueError(f"max_len {max_len} exceeds the model's rotary table "
+                             f"(max_position {model.cos_sin.shape[0]})")
         self.model, self.max_len, self.max_tree, self.propose = model, max_len, max_tree, propose
         cfg, dev = model.cfg, model.device
         self.block_size = block_size
@@ -182,9 +185,9 @@ class TreeDecoder:
         tree_kv = torch.empty(L, 2, R, hkv, D, dtype=self.kv.dtype, device=self.kv.device)
         logits = m.verify_step(ids, plan, tree_kv, self.kv, req.tables, req.ctx)
         chosen = torch.empty(R, dtype=torch.int32, device=m.device)
-        ops.process_logits(logits, row_request=plan.row_request, tokens=tokens, token_lens=req.ctx, prompt_lens=prompt_lens,
-                           draft_ids=ids, indptr=plan.indptr, tree_mask=plan.tree_mask, positions=plan.positions,
-                           out=logits, greedy=chosen, **rules)
+        ops.process_logits(logits, row_request=plan.row_request, tokens=tokens, token_lens=req.ctx,
+                           prompt_lens=prompt_lens, draft_ids=ids, indptr=plan.indptr, tree_mask=plan.tree_mask,
+                           positions=plan.positions, out=logits, greedy=chosen, **rules)
         done = ops.commit_tree(ids, chosen, par, plan.indptr, req.ctx, plan.slot_mapping, tree_kv=tree_kv,
                                kv_cache=self.kv, tokens=tokens)
         req.ctx = done.ctx_lens

@@ -63,8 +63,10 @@ def plan_step(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torc
     few blocks nobody gets one, rows without a block have slot -1, and the
     device status says so.  ``parents`` int32 [num_rows] (-1 for the root,
     index inside the tree otherwise) gives tree masks of ``max_tree`` bits and
-    depths; without it the rows are chains.  At most 16384 requests.  ``held`` and ``cursor`` may also
-    be ``out.held`` and ``out.cursor`` (state updated in place).
+    depths; without it the rows are chains.  At most 16384 requests.  ``held``
+    and ``cursor`` may also be ``out.held`` and ``out.cursor`` (state updated
+    in place).  Steps of more than 1024 rows or requests take 16 bytes of
+    scratch memory.
     """
     # more than 1024 rows or requests: a second launch updates the state
     count_launches(1 if max(num_rows, ctx_lens.numel()) <= 1024 else 2)
@@ -86,8 +88,13 @@ def paged_tree_attention(q: torch.Tensor, k_tree: torch.Tensor, v_tree: torch.Te
     request whose bit is set in ``tree_mask[r]`` (without a mask: the rows up
     to itself).  A row that sees nothing, and padding rows, give zeros.
     bf16 or fp16, head_dim 64 or 128, up to 128 query heads per KV head, a
-    positive ``scale``; head rows start at 16-byte boundaries.  ``k_tree`` /
-    ``v_tree`` ``[R, Hkv, D]`` hold the step's own K and V.  Probabilities are
+    positive ``scale``; head rows start at 16-byte boundaries.  Block sizes
+    that are no multiple of 8 tokens work, but many times slower.  ``k_tree`` /
+    ``v_tree`` ``[R, Hkv, D]`` hold the step's own K and V.  Contexts end with
+    the block table at the latest; block ids outside the cache read as zeros.
+    Each call takes scratch memory from torch's allocator for the records of
+    shared items: 4 x SMs x min(128, R x Hq / Hkv) x (4 D + 8) bytes, 39 MB at
+    most on 148 SMs.  Probabilities are
     rounded to the K/V type before the product with V (fp16: with all bits
     down to 2^-21 of the row's largest one, none below 2^-32); sums are fp32."""
     if scale is None:
@@ -129,12 +136,13 @@ def process_logits(logits: torch.Tensor, *, row_request: Optional[torch.Tensor] 
     rows to requests (-1: no rules but the grammar; None: row r is request r).
     ``bias_ids`` / ``bias_values`` [B, K]: ids below 0 are padding, an id
     listed twice gets the sum; at most 2047 a request.  ``tokens`` may be up to
-    2^19 wide (less the number of rows).  ``allowed`` int32 [A, ceil(V / 32)] holds bit
+    2^19 wide (less the number of rows); at most 65535 rows.  ``allowed`` int32 [A, ceil(V / 32)] holds bit
     masks over the columns, ``allowed_index`` [R] names each row's mask (-1:
     none).  With ``vocab_begin`` the columns are a shard of the vocabulary;
     ids outside it are ignored.  ``greedy`` int32 [R] receives the index of
     the largest value of ``out`` (lowest index of equal ones, the first NaN if
-    there is one) and ``greedy_val`` fp32 [R] the value."""
+    there is one) and ``greedy_val`` fp32 [R] the value; it takes 8 bytes of
+    scratch memory for each row and slice (1024 to 16384 entries) of it."""
     if out is None:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     count_launches(1 if greedy is None else 2)
